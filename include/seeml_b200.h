@@ -174,6 +174,111 @@ int seeml_b200_last_run_ms(seeml_b200_ctx* ctx, float* ms);
 int seeml_b200_xent_fwd_noalloc(const float* logits, const int32_t* labels, float* loss, float* probs,
                                 uint64_t rows, uint64_t classes, void* stream);
 
+/* ------------------------------------------------------------ vocabulary-row operators --
+ * No counterpart in the reference, whose losses are a mean over rows (loss.cc:43-58) and whose
+ * distillation reads a teacher's dense logits (loss.cc:90-140). These work on a [rows, vocab]
+ * matrix of logits that the caller owns, row r at logits + r * row_stride elements, in f32, bf16
+ * or f16: per-row scores of given tokens with the top alternatives (what a teacher's pass keeps),
+ * and distillation of a student from such entries, each with its gradient.
+ *
+ * All pointers are DEVICE pointers on the CURRENT device, aligned to their element, and outlive
+ * the call's kernels; `stream` is a cudaStream_t (NULL = the default stream). A call only launches
+ * kernels on that stream: no allocation, no synchronisation, no scratch shared between calls, so
+ * calls on several streams may overlap and any of them may be captured into a graph. Results do
+ * not depend on the launch: the same call gives the same bits. Arguments are checked before
+ * anything is launched. rows == 0 is a valid, empty call. Limits: rows <= 2^27, one row of logits
+ * <= 1.5 MiB, top_k <= 128.
+ *
+ * x is a row of logits, T the temperature, p = softmax(x / T). A logit of -inf is a masked token
+ * (p = 0). A row that is masked as a whole has log probabilities of -inf, entropy 0 and a zero
+ * gradient. A NaN or +inf among a row's logits makes the row's numbers NaN. */
+#define SEEML_B200_DTYPE_F32 0u
+#define SEEML_B200_DTYPE_BF16 1u
+#define SEEML_B200_DTYPE_F16 2u
+#define SEEML_B200_TOP_K_MAX 128u
+
+/* Token scores: of each row the log probability of one given token, the entropy of p, and the
+ * top_k most likely tokens with their log probabilities (greater logit first, ties and masked
+ * tokens by the lower index, NaN ahead of all). A negative label is a row without a token: its
+ * logprob is 0. A label >= vocab is not dereferenced; its logprob is NaN. */
+typedef struct seeml_b200_token_scores {
+  const void* logits;
+  const int32_t* labels;   /* [rows]; may be NULL when logprob is */
+  float* logprob;          /* [rows]; may be NULL */
+  float* entropy;          /* [rows]; may be NULL */
+  float* stats;            /* [rows, 2]: max x, sum exp((x - max x) / T); may be NULL */
+  float* top_logprob;      /* [rows, top_k]; may be NULL when top_k == 0 */
+  int32_t* top_id;         /* [rows, top_k]; may be NULL when top_k == 0 */
+  uint64_t rows, vocab, row_stride;
+  uint32_t dtype, top_k;
+  float temperature;
+  uint32_t reserved;       /* 0 */
+} seeml_b200_token_scores;
+int seeml_b200_token_scores_fwd(const seeml_b200_token_scores* d, void* stream);
+
+/* Gradient of sum_r (dlogprob[r] * logprob[r] + dentropy[r] * entropy[r]) with respect to the
+ * logits, from the stats and entropy of the forward call:
+ *   dlogits[j] = (dlogprob (1[j = label] - p_j) - dentropy p_j (ln p_j + entropy)) / T
+ * in the logits' type. dlogits may be the logits themselves (same pointer and stride); any other
+ * overlap is refused. A row whose upstream gradients are both 0 gets zeros and is not read. */
+typedef struct seeml_b200_token_scores_grad {
+  const void* logits;
+  const int32_t* labels;   /* [rows]; may be NULL when dlogprob is */
+  const float* stats;      /* [rows, 2] */
+  const float* entropy;    /* [rows]; may be NULL when dentropy is */
+  const float* dlogprob;   /* [rows]; NULL = zeros */
+  const float* dentropy;   /* [rows]; NULL = zeros; not both NULL */
+  void* dlogits;           /* row r at dlogits + r * grad_stride elements */
+  uint64_t rows, vocab, row_stride, grad_stride;
+  uint32_t dtype;
+  float temperature;
+} seeml_b200_token_scores_grad;
+int seeml_b200_token_scores_bwd(const seeml_b200_token_scores_grad* d, void* stream);
+
+/* Distillation from a teacher's top entries. Row r has top_k entries (token, value); an entry with
+ * a negative token is absent, lists may be ragged. Values are the teacher's log probabilities at
+ * the temperature (what token_scores_fwd returns). Without `tail` the teacher is the softmax of
+ * the present values (so unnormalised logits / T serve too): l = sum_i q_i (ln q_i - ln p_i). With
+ * `tail` q_i = exp(value) and the rest of the teacher's mass, q_t = max(0, 1 - sum q_i), is
+ * compared with the student's mass p_t on all tokens that no entry names:
+ * l += q_t (ln q_t - ln p_t); the term is left out where every unnamed token is masked.
+ *   row_loss[r] = l,   loss = scale * sum_r row_weight[r] * row_loss[r]
+ * (there is no T^2; put it into scale). With dlogits the gradient of `loss` with respect to the
+ * logits is written in the same pass, in the logits' type; dlogits may be the logits themselves.
+ * A row of weight 0 is not read: row_loss 0, gradient 0. A token named twice counts with the sum
+ * of its entries' q. An entry with a token >= vocab is not dereferenced; it makes the row NaN. */
+typedef struct seeml_b200_distill_topk {
+  const void* logits;
+  const int32_t* teacher_id;     /* [rows, top_k] */
+  const void* teacher_logprob;   /* [rows, top_k] of teacher_dtype */
+  const float* row_weight;       /* [rows]; NULL = ones */
+  float* row_loss;               /* [rows] */
+  float* loss;                   /* scalar; may be NULL */
+  float* saved;                  /* [rows, 4]: max and exp sum over unnamed tokens, over all; may be NULL */
+  void* dlogits;                 /* may be NULL; row r at dlogits + r * grad_stride elements */
+  uint64_t rows, vocab, row_stride, grad_stride;
+  uint32_t dtype, teacher_dtype, top_k, tail;
+  float temperature, scale;
+} seeml_b200_distill_topk;
+int seeml_b200_distill_topk_fwd(const seeml_b200_distill_topk* d, void* stream);
+
+/* Gradient of sum_r drow_loss[r] * row_loss[r] with respect to the logits, from `saved` of the
+ * forward call. A row whose drow_loss is 0 gets zeros and is not read. dlogits may be the logits
+ * themselves; any other overlap is refused. */
+typedef struct seeml_b200_distill_topk_grad {
+  const void* logits;
+  const int32_t* teacher_id;
+  const void* teacher_logprob;
+  const float* saved;            /* [rows, 4] */
+  const float* drow_loss;        /* [rows] */
+  void* dlogits;
+  uint64_t rows, vocab, row_stride, grad_stride;
+  uint32_t dtype, teacher_dtype, top_k, tail;
+  float temperature;
+  uint32_t reserved;             /* 0 */
+} seeml_b200_distill_topk_grad;
+int seeml_b200_distill_topk_bwd(const seeml_b200_distill_topk_grad* d, void* stream);
+
 /* ------------------------------------------------- data-parallel gradient sets --
  * No counterpart in the reference (single process). A gradient set is the list of
  * (arena offset, float count) pairs of the optimiser instructions' gradient

@@ -32,6 +32,30 @@ class TrainReport(C.Structure):
                 ("val_final_accuracy", f32), ("improved", i32)]
 
 
+class TokenScores(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "labels", "logprob", "entropy", "stats", "top_logprob", "top_id")] + \
+        [(n, u64) for n in ("rows", "vocab", "row_stride")] + \
+        [("dtype", u32), ("top_k", u32), ("temperature", f32), ("reserved", u32)]
+
+
+class TokenScoresGrad(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "labels", "stats", "entropy", "dlogprob", "dentropy", "dlogits")] + \
+        [(n, u64) for n in ("rows", "vocab", "row_stride", "grad_stride")] + [("dtype", u32), ("temperature", f32)]
+
+
+class DistillTopk(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "teacher_id", "teacher_logprob", "row_weight", "row_loss", "loss",
+                                  "saved", "dlogits")] + \
+        [(n, u64) for n in ("rows", "vocab", "row_stride", "grad_stride")] + \
+        [(n, u32) for n in ("dtype", "teacher_dtype", "top_k", "tail")] + [("temperature", f32), ("scale", f32)]
+
+
+class DistillTopkGrad(C.Structure):
+    _fields_ = [(n, vp) for n in ("logits", "teacher_id", "teacher_logprob", "saved", "drow_loss", "dlogits")] + \
+        [(n, u64) for n in ("rows", "vocab", "row_stride", "grad_stride")] + \
+        [(n, u32) for n in ("dtype", "teacher_dtype", "top_k", "tail")] + [("temperature", f32), ("reserved", u32)]
+
+
 STOP_FN = C.CFUNCTYPE(INT, vp)
 
 
@@ -76,6 +100,10 @@ SIGNATURES = {
     "seeml_b200_ctx_enable_timing": (INT, [vp, INT]),
     "seeml_b200_last_run_ms": (INT, [vp, C.POINTER(f32)]),
     "seeml_b200_xent_fwd_noalloc": (INT, [vp, vp, vp, vp, u64, u64, vp]),
+    "seeml_b200_token_scores_fwd": (INT, [C.POINTER(TokenScores), vp]),
+    "seeml_b200_token_scores_bwd": (INT, [C.POINTER(TokenScoresGrad), vp]),
+    "seeml_b200_distill_topk_fwd": (INT, [C.POINTER(DistillTopk), vp]),
+    "seeml_b200_distill_topk_bwd": (INT, [C.POINTER(DistillTopkGrad), vp]),
     "seeml_b200_grads_pack": (INT, [vp, vp, vp, u64, vp]),
     "seeml_b200_grads_unpack": (INT, [vp, vp, vp, u64, vp]),
     "seeml_b200_tree_sum": (INT, [vp, vp, u64, u64, f32]),

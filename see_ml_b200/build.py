@@ -32,8 +32,9 @@ EXTRA = {"kernels_mem.cu": ["-fmad=false"]}
 GXX_FLAGS = ["-O2", "-std=c++23", "-fPIC", "-pthread", "-I" + INCLUDE, "-I" + CSRC,
              "-I" + os.path.join(CUDA, "include"), "-Wall", "-Wextra", "-Wno-unused-parameter"]
 
-CU_SRCS = ["kernels_mem.cu", "kernels_gemm_simt.cu", "kernels_skinny.cu", "gemm_tc.cu", "backend.cu", "xent_noalloc.cu"]
-CC_SRCS = ["validate.cc", "dataset.cc", "engine.cc", "comm.cc"]
+CU_SRCS = ["kernels_mem.cu", "kernels_gemm_simt.cu", "kernels_skinny.cu", "gemm_tc.cu", "backend.cu", "xent_noalloc.cu",
+           "kernels_token.cu"]
+CC_SRCS = ["validate.cc", "dataset.cc", "engine.cc", "comm.cc", "token_ops.cc"]
 
 
 def _stale(src, obj, deps):

@@ -7,6 +7,8 @@
 #include <cstddef>
 #include <cstdint>
 
+#include "seeml_b200.h"
+
 namespace seeml_b200 {
 
 // Per-step optimiser scalars as the kernels read them (device memory, so that a
@@ -69,6 +71,17 @@ int kl_fwd(const float* s, const float* t, float* loss, float* ps, float* pt, si
 int kl_bwd(const float* ps, const float* pt, const float* seed, float* d, size_t N, size_t C,
            float T, cudaStream_t st);
 size_t loss_scratch_doubles(size_t rows_or_elems);
+
+// ---- vocabulary rows (no counterpart in the reference), kernels_token.cu -------------------
+// The descriptors are the C ABI's own, already checked (token_ops.cc); rows >= 1 except for
+// row_loss_sum. Each returns the number of kernels it launched, or a negative value when the
+// device refused an attribute or the launch (cudaGetLastError tells).
+int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st);
+int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st);
+int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st);   // row losses, saved, dlogits
+int distill_topk_bwd(const seeml_b200_distill_topk_grad& d, cudaStream_t st);
+// loss = scale * sum_r weight[r] * row_loss[r] in a fixed order; weight nullable, rows of weight 0 skipped
+int row_loss_sum(const float* row_loss, const float* weight, size_t rows, float scale, float* loss, cudaStream_t st);
 
 // ---- optimiser family (optimizer.cc:17-69) -------------------------------------------
 int clip_norm(float* g, size_t n, float max_norm, double* scratch, cudaStream_t st);

@@ -1,0 +1,477 @@
+"""Vocabulary-row operators (token scores, distillation from a teacher's top entries) against
+their 64-bit definitions, and their refusals."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import token_ref as R
+
+torch = pytest.importorskip("torch")
+gpu = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+# ---- refusals that need no device ------------------------------------------------------------
+def _rc(fn, d):
+    from see_ml_b200 import _lib as L
+    return getattr(L.lib(), fn)(C.byref(d) if d is not None else None, None), L.last_error()
+
+
+def _scores(**kw):
+    from see_ml_b200 import _lib as L
+    base = dict(logits=1024, labels=1024, logprob=1024, entropy=1024, stats=1024, top_logprob=1024, top_id=1024, rows=2,
+                vocab=64, row_stride=64, dtype=0, top_k=4, temperature=1.0, reserved=0)
+    return L.TokenScores(**{**base, **kw})
+
+
+def _scores_grad(**kw):
+    from see_ml_b200 import _lib as L
+    base = dict(logits=1024, labels=1024, stats=1024, entropy=1024, dlogprob=1024, dentropy=1024, dlogits=1024, rows=2,
+                vocab=64, row_stride=64, grad_stride=64, dtype=0, temperature=1.0)
+    return L.TokenScoresGrad(**{**base, **kw})
+
+
+def _distill(**kw):
+    from see_ml_b200 import _lib as L
+    base = dict(logits=1024, teacher_id=1024, teacher_logprob=1024, row_weight=1024, row_loss=1024, loss=1024, saved=1024,
+                dlogits=1024, rows=2, vocab=64, row_stride=64, grad_stride=64, dtype=0, teacher_dtype=0, top_k=4, tail=0,
+                temperature=1.0, scale=1.0)
+    return L.DistillTopk(**{**base, **kw})
+
+
+def _distill_grad(**kw):
+    from see_ml_b200 import _lib as L
+    base = dict(logits=1024, teacher_id=1024, teacher_logprob=1024, saved=1024, drow_loss=1024, dlogits=1024, rows=2,
+                vocab=64, row_stride=64, grad_stride=64, dtype=0, teacher_dtype=0, top_k=4, tail=0, temperature=1.0, reserved=0)
+    return L.DistillTopkGrad(**{**base, **kw})
+
+
+MATRIX = [(dict(dtype=3), "unknown dtype"), (dict(vocab=0), "empty vocabulary"), (dict(rows=(1 << 27) + 1), "2^27 rows"),
+          (dict(vocab=393217, row_stride=400000), "at most 393216"), (dict(row_stride=63), "row stride"),
+          (dict(dtype=1, vocab=786433, row_stride=800000), "at most 786432"),
+          (dict(row_stride=1 << 58), "row stride"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
+          (dict(temperature=math.nan), "temperature"), (dict(temperature=math.inf), "temperature"),
+          (dict(temperature=1e-45), "temperature"), (dict(logits=None), "logits is null"), (dict(logits=4098), "logits is not aligned")]
+GRADIENT = [(dict(grad_stride=63), "gradient stride"), (dict(grad_stride=1 << 58), "gradient stride"),
+            (dict(dlogits=1028), "overlaps"), (dict(dlogits=1024 + 252, row_stride=127, grad_stride=127), "overlaps"),
+            (dict(grad_stride=65), "overlaps"), (dict(dlogits=1024 + 256), "overlaps")]
+TEACHER = [(dict(top_k=0), "top_k"), (dict(top_k=129), "top_k"), (dict(teacher_dtype=3), "teacher dtype"),
+           (dict(teacher_id=None), "teacher_id is null"), (dict(teacher_logprob=None), "teacher_logprob is null")]
+REFUSED = (
+    [("seeml_b200_token_scores_fwd", _scores, kw, m) for kw, m in MATRIX + [
+        (dict(top_k=129), "top_k"), (dict(top_k=65), "top_k"), (dict(reserved=1), "reserved"), (dict(labels=None), "labels is null"),
+        (dict(top_id=None), "top_id is null"), (dict(top_logprob=None), "top_logprob is null"),
+        (dict(logprob=None, entropy=None, stats=None, top_k=0), "no output"), (dict(stats=1025), "stats is not aligned")]] +
+    [("seeml_b200_token_scores_bwd", _scores_grad, kw, m) for kw, m in MATRIX + GRADIENT + [
+        (dict(dlogprob=None, dentropy=None), "neither"), (dict(labels=None), "labels is null"), (dict(stats=None), "stats is null"),
+        (dict(entropy=None), "entropy is null"), (dict(dlogits=None), "dlogits is null")]] +
+    [("seeml_b200_distill_topk_fwd", _distill, kw, m) for kw, m in MATRIX + GRADIENT + TEACHER + [
+        (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"), (dict(row_loss=None), "row_loss is null")]] +
+    [("seeml_b200_distill_topk_bwd", _distill_grad, kw, m) for kw, m in MATRIX + GRADIENT + TEACHER + [
+        (dict(saved=None), "saved is null"), (dict(drow_loss=None), "drow_loss is null"), (dict(dlogits=None), "dlogits is null"),
+        (dict(reserved=1), "reserved")]])
+
+
+@pytest.mark.parametrize("fn,make,kw,message", REFUSED, ids=lambda v: None if callable(v) else str(v).replace("seeml_b200_", ""))
+def test_refused_before_any_launch(backend_lib, fn, make, kw, message):
+    rc, err = _rc(fn, make(**kw))
+    assert rc != 0 and err.startswith("UpdateEngine: ") and message in err, err
+
+
+@pytest.mark.parametrize("fn", ["seeml_b200_token_scores_fwd", "seeml_b200_token_scores_bwd", "seeml_b200_distill_topk_fwd",
+                                "seeml_b200_distill_topk_bwd"])
+def test_null_descriptor_is_refused(backend_lib, fn):
+    rc, err = _rc(fn, None)
+    assert rc != 0 and "null descriptor" in err
+
+
+def test_empty_calls_need_no_device(backend_lib):
+    for fn, d in (("seeml_b200_token_scores_fwd", _scores(rows=0)), ("seeml_b200_token_scores_bwd", _scores_grad(rows=0)),
+                  ("seeml_b200_distill_topk_fwd", _distill(rows=0, loss=None)),
+                  ("seeml_b200_distill_topk_bwd", _distill_grad(rows=0))):
+        assert _rc(fn, d)[0] == 0, fn
+
+
+def test_python_refuses_what_the_library_cannot_see(backend_lib):
+    from see_ml_b200 import _lib as L, token_ops as T
+    x = torch.zeros(4, 8)
+    with pytest.raises(L.BackendError, match="device memory"):
+        T.token_scores(x)
+    with pytest.raises(L.BackendError, match="rows, vocab"):
+        T.token_scores(torch.zeros(8))
+
+
+# ---- on the device ---------------------------------------------------------------------------
+def _logits(rng, rows, V, dtype, pad=0, std=3.0, masked=0.0):
+    x = rng.standard_normal((rows, V)) * std
+    if masked:
+        hide = rng.random((rows, V)) < masked
+        hide[np.arange(rows), rng.integers(0, V, rows)] = False
+        x[hide] = -np.inf
+    buf = torch.full((rows + 1, V + pad), 7.0, dtype=dtype, device="cuda")
+    view = buf[:rows, :V]
+    view.copy_(torch.from_numpy(x))
+    return buf, view
+
+
+def _f64(t):
+    return t.double().cpu().numpy()
+
+
+def _close(got, want, bound, dtype, what):
+    got, want = _f64(got), np.array(want, np.float64)
+    want[np.abs(want) > torch.finfo(dtype).max] *= np.inf      # beyond the type
+    nonfinite = ~np.isfinite(want)
+    np.testing.assert_array_equal(got[nonfinite], want[nonfinite], err_msg=what)
+    err = np.abs(np.where(nonfinite, 0.0, got - np.where(nonfinite, 0.0, want)))
+    bar = np.where(nonfinite, 0.0, bound + R.half_step(dtype) * np.abs(np.where(nonfinite, 0.0, want)) * (1 + 2 ** -6)) + R.floor_of(dtype)
+    bad = ~(err <= bar)
+    assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} out; worst {np.max(err / bar):.3f} of the bound"
+
+
+SHAPES = [  # rows, vocab, dtype, pad, temperature, masked
+    (1, 1, F32, 0, 1.0, 0.0), (3, 2, F16, 1, 0.5, 0.0), (5, 7, BF16, 0, 1.0, 0.3), (2, 33, F32, 3, 2.0, 0.5),
+    (9, 255, F16, 0, 1.0, 0.0), (4, 1000, F32, 0, 0.7, 0.9), (3, 4097, BF16, 5, 1.5, 0.2), (1, 5000, F32, 0, 1.0, 0.0),
+    (300, 513, F32, 0, 1.0, 0.1), (7, 32000, F32, 0, 1.0, 0.0), (2, 32000, BF16, 0, 0.8, 0.3), (5, 50001, F16, 7, 1.0, 0.0),
+    (1, 131072, BF16, 0, 1.0, 0.0), (3, 100003, F32, 0, 2.0, 0.6), (2, 393216, F32, 0, 1.0, 0.0), (1, 786432, F16, 0, 1.0, 0.0)]
+
+
+def _ids(v):
+    return str(v).replace("torch.", "")
+
+
+@gpu
+@pytest.mark.parametrize("rows,V,dtype,pad,T,masked", SHAPES, ids=_ids)
+@pytest.mark.parametrize("k", [0, 1, 20, 128])
+def test_token_scores(backend_lib, rows, V, dtype, pad, T, masked, k):
+    from see_ml_b200 import token_ops as ops
+    k = min(k, V)
+    rng = np.random.default_rng(V * 31 + k)
+    _, x = _logits(rng, rows, V, dtype, pad, masked=masked)
+    labels = rng.integers(-1, V, rows).astype(np.int32)
+    s = ops.token_scores(x, torch.from_numpy(labels).cuda(), top_k=k, temperature=T)
+    lp, h, tlp, tid = R.scores(_f64(x), labels, k, T)
+    d = R.delta(V)
+    _close(s.logprob, lp, d, F32, "logprob")
+    _close(s.entropy, h, 2 * (1 + math.log(V)) * d, F32, "entropy")
+    _close(s.stats[:, 0], _f64(x).max(1), 0.0, F32, "max")
+    if k:
+        np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+        _close(s.top_logprob, tlp, d, F32, "top_logprob")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=_ids)
+@pytest.mark.parametrize("V,k", [(40, 40), (3000, 17), (32000, 128), (100003, 100)])
+@pytest.mark.parametrize("shape", ["constant", "ascending", "descending", "few", "one_slice", "zeros_of_both_signs", "lowest"])
+def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape):
+    """Ties go to the lower index, whatever the order and wherever the great values lie."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V + k)
+    j = np.arange(V)
+    x = {"constant": np.full(V, 1.5), "ascending": j / V * 8, "descending": -j / V * 8, "few": rng.integers(0, 3, V) * 1.0,
+         "one_slice": np.where((j // 8) % 512 == 3, 5.0 + rng.standard_normal(V), rng.standard_normal(V)),
+         "zeros_of_both_signs": np.where(j % 2, 0.0, -0.0), "lowest": np.full(V, torch.finfo(dtype).min)}[shape]
+    t = torch.from_numpy(np.stack([x, x[::-1].copy()])).to(dtype).cuda()
+    s = ops.token_scores(t, None, top_k=k)
+    _, h, tlp, tid = R.scores(_f64(t), None, k, 1.0)
+    np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+    _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
+    _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
+
+
+@gpu
+@pytest.mark.parametrize("V", [5, 700, 32000])
+def test_rows_that_are_masked_or_not_finite(backend_lib, V):
+    from see_ml_b200 import token_ops as ops
+    x = np.random.default_rng(V).standard_normal((7, V))
+    x[0] = -np.inf                           # nothing left
+    x[1, 2] = np.nan
+    x[2, 3] = np.inf
+    x[3, 1:] = -np.inf                       # one token left
+    x[4, ::2] = -3.4e38
+    x[5, 1] = np.nan
+    x[5, 4] = np.nan
+    t = torch.from_numpy(x).float().cuda()
+    labels = np.array([1, 0, 0, 0, 1, 3, V + 5], np.int32)
+    s = ops.token_scores(t, torch.from_numpy(labels).cuda(), top_k=4, temperature=0.5)
+    lp, h, tlp, tid = R.scores(_f64(t), labels, 4, 0.5)
+    np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+    _close(s.logprob, lp, R.delta(V), F32, "logprob")
+    _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
+    _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
+    ones = torch.ones(7, device="cuda")
+    g = _f64(ops.token_scores_backward(t, torch.from_numpy(labels).cuda(), s.stats, s.entropy, ones, ones, temperature=0.5))
+    assert (g[0] == 0).all() and np.isnan(g[1]).all() and np.isnan(g[2]).all() and np.isnan(g[6]).all()
+    assert (g[3] == 0).all() and np.isfinite(g[4]).all() and np.isnan(g[5]).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows,V,dtype,pad,T,masked", SHAPES, ids=_ids)
+@pytest.mark.parametrize("parts", ["both", "logprob", "entropy"])
+def test_token_scores_gradient(backend_lib, rows, V, dtype, pad, T, masked, parts):
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V * 7 + rows)
+    _, x = _logits(rng, rows, V, dtype, pad, masked=masked)
+    labels = rng.integers(-1, V, rows).astype(np.int32)
+    gl, gh = rng.standard_normal((2, rows)).astype(np.float32)
+    gl[rows // 2] = gh[rows // 2] = 0.0
+    lab = torch.from_numpy(labels).cuda()
+    s = ops.token_scores(x, lab, temperature=T)
+    up = [torch.from_numpy(v).cuda() for v in (gl, gh)]
+    g = ops.token_scores_backward(x, lab, s.stats, s.entropy, up[0] if parts != "entropy" else None,
+                                  up[1] if parts != "logprob" else None, temperature=T)
+    want, err = R.scores_grad(_f64(x), labels, gl.astype(np.float64) * (parts != "entropy"),
+                              gh.astype(np.float64) * (parts != "logprob"), T)
+    _close(g, want, err, dtype, "dlogits")
+
+
+def _teacher(rng, rows, V, K, dtype, absent=0.0):
+    ids = np.stack([rng.permutation(V)[:K] if V < 200000 else np.unique(rng.integers(0, V, 4 * K))[:K] for _ in range(rows)])
+    if K > V:
+        ids = np.concatenate([ids, np.full((rows, K - V), -1)], 1)
+    v = rng.standard_normal((rows, K)) * 1.5
+    v = v - np.log(np.exp(v).sum(1, keepdims=True)) + math.log(0.9)
+    ids = np.where(rng.random((rows, K)) < absent, -1, ids).astype(np.int32)
+    return torch.from_numpy(ids).cuda(), torch.from_numpy(v).to(dtype).cuda()
+
+
+@gpu
+@pytest.mark.parametrize("rows,V,dtype,pad,T,masked", SHAPES, ids=_ids)
+@pytest.mark.parametrize("K,tail,tdtype", [(1, True, F32), (17, False, BF16), (128, True, F16), (33, True, F32)], ids=_ids)
+def test_distill(backend_lib, rows, V, dtype, pad, T, masked, K, tail, tdtype):
+    """Loss, its gradient in the same pass, and the gradient of a pass of its own."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V * 13 + K)
+    buf, x = _logits(rng, rows, V, dtype, pad, masked=masked if K < 17 else 0.0)
+    ids, v = _teacher(rng, rows, V, K, tdtype, absent=0.1)
+    if masked and K < 17:        # a masked token that the teacher names makes the loss infinite
+        x.scatter_(1, ids.clamp(min=0).long(), 1.0)
+    before = buf.clone()
+    w = rng.integers(0, 3, rows).astype(np.float32)
+    scale = 0.25
+    wt = torch.from_numpy(w).cuda()
+    r = ops.distill_topk(x, ids, v, row_weight=wt, scale=scale, temperature=T, tail=tail, grad=True, saved=True)
+    loss, lerr, grad, gerr = R.distill(_f64(x), ids.cpu().numpy(), _f64(v), T, tail)
+    loss, lerr = np.where(w == 0, 0.0, loss), np.where(w == 0, 0.0, lerr)
+    _close(r.row_loss, loss, lerr, F32, "row_loss")
+    _close(r.loss, scale * (w * loss).sum(), scale * (w * (lerr + np.abs(loss) * R.U)).sum(), F32, "loss")
+    up = (scale * w.astype(np.float64))[:, None]
+    _close(r.dlogits, grad * up, gerr * up, dtype, "dlogits")
+    d = torch.from_numpy((w * scale).astype(np.float32)).cuda()
+    g = ops.distill_topk_backward(x, ids, v, r.saved, d, temperature=T, tail=tail)
+    _close(g, grad * up, gerr * up, dtype, "dlogits of the backward call")
+    assert torch.equal(buf, before)
+    alone = ops.distill_topk(x, ids, v, row_weight=wt, scale=scale, temperature=T, tail=tail)
+    assert torch.equal(alone.row_loss, r.row_loss) and torch.equal(alone.loss, r.loss)
+    inplace = ops.distill_topk(x, ids, v, row_weight=wt, scale=scale, temperature=T, tail=tail, out=x)
+    assert inplace.dlogits is x and torch.equal(x, r.dlogits) and torch.equal(inplace.row_loss, r.row_loss)
+    assert torch.equal(buf[rows], before[rows]) and torch.equal(buf[:, V:], before[:, V:])
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("V", [9, 3000, 70001])
+def test_distill_of_awkward_rows(backend_lib, V, tail):
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((10, V)) * 2
+    ids = np.stack([rng.permutation(V)[:6] for _ in range(10)]).astype(np.int32)
+    v = np.log(np.tile([0.4, 0.2, 0.1, 0.1, 0.05, 0.05], (10, 1)))
+    ids[0] = -1                       # no entry
+    v[1] = -np.inf                    # entries without mass
+    ids[2] = ids[2, 0]                # one token named by all
+    ids[3, 4] = ids[3, 1]             # and by two
+    v[4, 2] = -np.inf                 # a named token without mass
+    x[5] = -np.inf                    # nothing left of the student
+    x[6, ids[6, 3]] = -np.inf         # the student masks a token that the teacher wants
+    ids[7, 0] = V                     # beyond the vocabulary
+    x[8] = -300.0                     # the unnamed tokens vanish beside the named ones in f32
+    x[8, ids[8]] = 20.0
+    ids[9, 3:] = -1
+    t = torch.from_numpy(x).float().cuda()
+    vt = torch.from_numpy(v).float().cuda()
+    it = torch.from_numpy(ids).cuda()
+    good = [i for i in range(10) if i != 7]
+    for out in (None, t.clone()):
+        src = t if out is None else out
+        r = ops.distill_topk(src, it, vt, tail=tail, grad=True, saved=True, out=out)
+        loss, lerr, grad, gerr = R.distill(_f64(t)[good], ids[good], _f64(vt)[good], 1.0, tail)
+        _close(r.row_loss[good], loss, lerr, F32, "row_loss")
+        _close(r.dlogits[good], grad, gerr, F32, "dlogits")
+        assert torch.isnan(r.row_loss[7]) and torch.isnan(r.dlogits[7]).all()
+    g = ops.distill_topk_backward(t, it, vt, r.saved, torch.ones(10, device="cuda"), tail=tail)
+    _close(g[good], grad, gerr, F32, "dlogits of the backward call")
+    assert torch.isnan(g[7]).all()
+    x[5, 0] = np.nan                  # a row of weight 0 is not looked at, another is
+    t = torch.from_numpy(x).float().cuda()
+    w = torch.ones(10, device="cuda")
+    r = ops.distill_topk(t, it, vt, tail=tail, grad=True, row_weight=w)
+    assert torch.isnan(r.row_loss[5]) and torch.isnan(r.dlogits[5]).all() and torch.isnan(r.loss)
+    w[5] = w[6] = w[7] = 0.0
+    r = ops.distill_topk(t, it, vt, tail=tail, grad=True, row_weight=w)
+    assert (r.row_loss[5:8] == 0).all() and (r.dlogits[5:8] == 0).all() and torch.isfinite(r.loss)
+
+
+@gpu
+@pytest.mark.parametrize("tail", [False, True])
+def test_gradients_against_differences(backend_lib, tail):
+    """Central differences of the kernels' own losses: truncation h^2 / 6 |f'''| <= h^2 / T^3, rounding of the two
+    values delta / h each."""
+    from see_ml_b200 import token_ops as ops
+    V, T, h = 37, 1.3, 2.0 ** -6
+    rng = np.random.default_rng(5)
+    x = torch.from_numpy(rng.standard_normal((1, V))).float().cuda()
+    steps = torch.cat([x + h * torch.eye(V, device="cuda"), x - h * torch.eye(V, device="cuda")])
+    width = (steps[:V] - steps[V:]).diagonal()
+    ids, v = _teacher(rng, 1, V, 6, F32)
+    r = ops.distill_topk(x, ids, v, temperature=T, tail=tail, grad=True)
+    f = ops.distill_topk(steps, ids.expand(2 * V, -1).contiguous(), v.expand(2 * V, -1).contiguous(), temperature=T, tail=tail).row_loss
+    lab = torch.tensor([4], dtype=torch.int32, device="cuda")
+    s = ops.token_scores(x, lab, temperature=T)
+    one = torch.ones(1, device="cuda")
+    g = ops.token_scores_backward(x, lab, s.stats, s.entropy, one, -one, temperature=T)
+    f2 = ops.token_scores(steps, lab.expand(2 * V).contiguous(), temperature=T)
+    bar = h * h / T ** 3 * (2 + math.log(V)) + 2 * (2 + 2 * math.log(V)) * R.delta(V) / h
+    assert ((f[:V] - f[V:]) / width - r.dlogits[0]).abs().max().item() <= bar
+    f2 = f2.logprob - f2.entropy
+    assert ((f2[:V] - f2[V:]) / width - g[0]).abs().max().item() <= bar
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V", [(BF16, 4097), (F32, 1000), (F16, 32001)], ids=_ids)
+@pytest.mark.parametrize("xo,go,xs,gs", [(0, 0, 0, 0), (1, 0, 3, 0), (0, 5, 0, 8), (3, 3, 7, 7), (8, 2, 1, 9)])
+def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs):
+    """Rows that start anywhere, gradients whose rows start elsewhere; nothing beside them is touched."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V + xo)
+    rows = 5
+    xb = torch.zeros(16 + rows * (V + xs), dtype=dtype, device="cuda")
+    x = xb[xo:xo + rows * (V + xs)].view(rows, V + xs)[:, :V]
+    x.copy_(torch.from_numpy(rng.standard_normal((rows, V)) * 2))
+    gb = torch.full((16 + rows * (V + gs),), 3.0, dtype=dtype, device="cuda")
+    g = gb[go:go + rows * (V + gs)].view(rows, V + gs)[:, :V]
+    ids, v = _teacher(rng, rows, V, 9, F32)
+    lab = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    one = torch.ones(rows, device="cuda")
+    flat = x.contiguous()
+    s0, s1 = ops.token_scores(flat, lab, top_k=9), ops.token_scores(x, lab, top_k=9)
+    assert torch.equal(s0.top_id, s1.top_id)
+    _close(s1.logprob, _f64(s0.logprob), 2 * R.delta(V), F32, "logprob")
+    loss, lerr, grad, gerr = R.distill(_f64(x), ids.cpu().numpy(), _f64(v), 1.0, True)
+    r = ops.distill_topk(x, ids, v, tail=True, out=g, saved=True)
+    _close(r.row_loss, loss, lerr, F32, "row_loss")
+    for call in (lambda: None, lambda: ops.distill_topk_backward(x, ids, v, r.saved, one, tail=True, out=g.zero_())):
+        call()
+        _close(g, grad, gerr, dtype, "dlogits")
+        edge = gb.clone()
+        edge[go:go + rows * (V + gs)].view(rows, V + gs)[:, :V] = 3.0
+        assert (edge == 3.0).all()
+    want, err = R.scores_grad(_f64(x), np.zeros(rows, np.int32), np.ones(rows), -np.ones(rows), 1.0)
+    ops.token_scores_backward(x, lab, s1.stats, s1.entropy, one, -one, out=g.zero_())
+    _close(g, want, err, dtype, "dlogits of the scores")
+
+
+@gpu
+def test_rows_beyond_32_bits_of_offset(backend_lib):
+    from see_ml_b200 import token_ops as ops
+    rows, V, stride = 3, 1001, (1 << 31) + 8
+    buf = torch.empty(2 * stride + V, dtype=BF16, device="cuda")
+    x = buf.as_strided((rows, V), (stride, 1))
+    rng = np.random.default_rng(0)
+    x.copy_(torch.from_numpy(rng.standard_normal((rows, V)) * 2))
+    flat = x.contiguous()
+    lab = torch.arange(rows, dtype=torch.int32, device="cuda")
+    ids, v = _teacher(rng, rows, V, 5, F32)
+    a, b = ops.token_scores(x, lab, top_k=5), ops.token_scores(flat, lab, top_k=5)
+    assert torch.equal(a.top_id, b.top_id)
+    _close(a.logprob, _f64(b.logprob), 2 * R.delta(V), F32, "logprob")
+    _, _, grad, gerr = R.distill(_f64(flat), ids.cpu().numpy(), _f64(v), 1.0, True)
+    ops.distill_topk(x, ids, v, tail=True, out=x)
+    _close(x, grad, gerr, BF16, "dlogits in place")
+
+
+@gpu
+def test_interleaved_gradient_rows(backend_lib):
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(3)
+    both = torch.zeros(6, 2 * 500, device="cuda")
+    x, g = both[:, :500], both[:, 500:]
+    x.copy_(torch.from_numpy(rng.standard_normal((6, 500))))
+    ids, v = _teacher(rng, 6, 500, 4, F32)
+    _, _, grad, gerr = R.distill(_f64(x), ids.cpu().numpy(), _f64(v), 1.0, False)
+    _close(ops.distill_topk(x, ids, v, out=g).dlogits, grad, gerr, F32, "dlogits")
+
+
+@gpu
+def test_device_refusals(backend_lib):
+    from see_ml_b200 import _lib as L, token_ops as ops
+    x = torch.zeros(4, 64, device="cuda")
+    ids, v = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, 2, device="cuda")
+    for bad in (lambda: ops.token_scores(x.double()), lambda: ops.token_scores(x.t()), lambda: ops.token_scores(x[:1].expand(4, -1)),
+                lambda: ops.token_scores(x, torch.zeros(4, dtype=torch.int64, device="cuda")),
+                lambda: ops.token_scores(x, torch.zeros(4, dtype=torch.int32)), lambda: ops.token_scores(x, top_k=65),
+                lambda: ops.token_scores(x, temperature=0.0), lambda: ops.distill_topk(x, ids.long(), v),
+                lambda: ops.distill_topk(x, ids[:3], v), lambda: ops.distill_topk(x, ids, v, out=x.half()),
+                lambda: ops.distill_topk(x, ids, v.t().contiguous().t()), lambda: ops.distill_topk(x, ids, v, scale=math.inf),
+                lambda: ops.distill_topk(x[:, :32], ids, v, out=x[:, 1:33]),
+                lambda: ops.distill_topk(x, ids, None)):
+        with pytest.raises(L.BackendError, match="^UpdateEngine: "):
+            bad()
+    host = np.zeros(256, np.float32)
+    rc, err = _rc("seeml_b200_token_scores_fwd", _scores(logits=x.data_ptr(), labels=host.ctypes.data, top_k=0, entropy=None,
+                                                         stats=None, logprob=v.data_ptr()))
+    assert rc != 0 and "labels" in err
+    empty = ops.distill_topk(x[:0], ids[:0], v[:0], grad=True)
+    assert empty.loss.item() == 0.0 and empty.dlogits.shape == (0, 64)
+    assert ops.token_scores(x[:0], ids[:0, 0], top_k=3).top_id.shape == (0, 3)
+
+
+@gpu
+def test_streams_and_graphs_give_the_same_bits(backend_lib):
+    """The calls of a step on two streams at once and in two captured graphs: no scratch is shared."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(1)
+    rows, V, k = 40, 20011, 24
+    xs = [torch.from_numpy(rng.standard_normal((rows, V)) * 2).to(BF16).cuda() for _ in range(2)]
+    lab = torch.arange(rows, dtype=torch.int32, device="cuda")
+    one = torch.ones(rows, device="cuda")
+
+    def step(teacher, student):
+        s = ops.token_scores(teacher, lab, top_k=k)
+        r = ops.distill_topk(student, s.top_id, s.top_logprob, scale=1 / rows, tail=True, grad=True)
+        g = ops.token_scores_backward(teacher, lab, s.stats, s.entropy, one, -one)
+        return [s.logprob, s.entropy, s.top_id, s.top_logprob, r.loss, r.row_loss, r.dlogits, g]
+
+    want = [[t.clone() for t in step(xs[0], xs[1])], [t.clone() for t in step(xs[1], xs[0])]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] = step(xs[i], xs[1 - i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(xs[i], xs[1 - i]))
+        graphs.append(g)
+    for _ in range(2):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    a, b = xs[0].clone(), xs[1].clone()
+    xs[0].copy_(b)
+    xs[1].copy_(a)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want[1], outs[0]))
