@@ -187,7 +187,7 @@ int seeml_b200_xent_fwd_noalloc(const float* logits, const int32_t* labels, floa
  * calls on several streams may overlap and any of them may be captured into a graph. Results do
  * not depend on the launch: the same call gives the same bits. Arguments are checked before
  * anything is launched. rows == 0 is a valid, empty call. Limits: rows <= 2^27, one row of logits
- * <= 1.5 MiB, top_k <= 128.
+ * <= 1.5 MiB, all of them <= 2^44 bytes, top_k <= 128.
  *
  * x is a row of logits, T the temperature, p = softmax(x / T). A logit of -inf is a masked token
  * (p = 0). A row that is masked as a whole has log probabilities of -inf, entropy 0 and a zero
@@ -220,7 +220,7 @@ int seeml_b200_token_scores_fwd(const seeml_b200_token_scores* d, void* stream);
  * logits, from the stats and entropy of the forward call:
  *   dlogits[j] = (dlogprob (1[j = label] - p_j) - dentropy p_j (ln p_j + entropy)) / T
  * in the logits' type. dlogits may be the logits themselves (same pointer and stride); any other
- * overlap is refused. A row whose upstream gradients are both 0 gets zeros and is not read. */
+ * overlap is refused. A row whose upstream gradients are both 0 gets zeros, whatever its logits. */
 typedef struct seeml_b200_token_scores_grad {
   const void* logits;
   const int32_t* labels;   /* [rows]; may be NULL when dlogprob is */

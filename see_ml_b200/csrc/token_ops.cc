@@ -15,6 +15,7 @@ namespace {
 
 constexpr uint64_t kMaxRows = 1ull << 27;          // rows x 8 blocks stay below the grid's 2^31
 constexpr uint64_t kMaxRowBytes = 3ull << 19;      // 1.5 MiB: eight blocks of a cluster hold 192 KiB each
+constexpr uint64_t kMaxBytes = 1ull << 44;          // a grid of one block per 16 KiB fits
 constexpr uint64_t kMaxElems = 1ull << 58;          // rows * stride: byte offsets stay below 2^63
 
 uint64_t elem_bytes(uint32_t dtype) { return dtype == SEEML_B200_DTYPE_F32 ? 4 : 2; }
@@ -65,6 +66,7 @@ int check_matrix(const char* op, uint64_t rows, uint64_t vocab, uint64_t stride,
   if (vocab > kMaxRowBytes / elem_bytes(dtype))
     return fail(unit + "a row holds at most " + std::to_string(kMaxRowBytes / elem_bytes(dtype)) +
                 " logits of this type (got " + std::to_string(vocab) + ")");
+  if (rows * (vocab * elem_bytes(dtype)) > kMaxBytes) return fail(unit + "more than 2^44 bytes of logits");
   if (stride < vocab || stride > kMaxElems / (rows ? rows : 1))
     return fail(unit + "row stride " + std::to_string(stride) + " is below vocab or beyond the address space");
   if (!(temperature > 0.0f) || std::isinf(temperature) || std::isinf(1.0f / temperature))

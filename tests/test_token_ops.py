@@ -51,7 +51,7 @@ def _distill_grad(**kw):
 MATRIX = [(dict(dtype=3), "unknown dtype"), (dict(vocab=0), "empty vocabulary"), (dict(rows=(1 << 27) + 1), "2^27 rows"),
           (dict(vocab=393217, row_stride=400000), "at most 393216"), (dict(row_stride=63), "row stride"),
           (dict(dtype=1, vocab=786433, row_stride=800000), "at most 786432"),
-          (dict(row_stride=1 << 58), "row stride"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
+          (dict(row_stride=1 << 58), "row stride"), (dict(rows=1 << 27, vocab=1 << 16, row_stride=1 << 16), "2^44 bytes"), (dict(temperature=0.0), "temperature"), (dict(temperature=-1.0), "temperature"),
           (dict(temperature=math.nan), "temperature"), (dict(temperature=math.inf), "temperature"),
           (dict(temperature=1e-45), "temperature"), (dict(logits=None), "logits is null"), (dict(logits=4098), "logits is not aligned")]
 GRADIENT = [(dict(grad_stride=63), "gradient stride"), (dict(grad_stride=1 << 58), "gradient stride"),
