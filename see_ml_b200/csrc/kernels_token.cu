@@ -28,8 +28,7 @@ constexpr int kClusterMax = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.6931471805599453;
 constexpr int kTopMax = SEEML_B200_TOP_K_MAX;
-constexpr int kCand = 1024;                 // candidates of the selection: kClusterMax * kTopMax fit
-static_assert(kCand >= kClusterMax * kTopMax && kTopMax <= kThreads, "selection buffers");
+static_assert(kTopMax <= kThreads, "a thread per entry, and as many maxima as the selection has to bound");
 
 __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fc00000); }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -134,71 +133,81 @@ __device__ __forceinline__ float load_as_f32(const void* p, uint32_t dtype, size
 
 // ---- one block's share of a row ------------------------------------------------------------------
 // The row is cut into the 16-byte vectors of its memory: vector v holds elements v*E - phase ...
-// +E-1, the first and the last may hang over the row's ends. Block `rank` of the cluster owns
-// vectors [rank*share, rank*share + n); thread t owns its vectors t, t + kThreads, ...
+// +E-1, the first and the last may hang over the row's ends. Block `rank` of the row owns vectors
+// [rank*share, rank*share + n); thread t owns its vectors t, t + kThreads, ... Vectors [lo, hi) of
+// the share lie inside the row as a whole.
 template <class T>
 struct Share {
   static constexpr int E = Ty<T>::E;
   const T* x;            // the row
-  uint32_t V, phase, first, n;
+  uint32_t V, phase, first, n, lo, hi;
   __device__ __forceinline__ Share(const void* base, size_t row, size_t stride, uint32_t V_, uint32_t share, uint32_t rank)
       : x(static_cast<const T*>(base) + row * stride), V(V_) {
     phase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T);
     const uint32_t nvec = (V + phase + E - 1) / E;
     first = rank * share;
     n = nvec <= first ? 0u : (nvec - first < share ? nvec - first : share);
+    lo = first == 0 && phase ? 1u : 0u;
+    hi = n && (first + n) * E - phase > V ? n - 1 : n;
   }
   // element index of vector i's first element (negative in a vector that hangs over the start)
   __device__ __forceinline__ int elem(uint32_t i) const { return static_cast<int>((first + i) * E) - static_cast<int>(phase); }
-  __device__ __forceinline__ bool whole(int j) const { return j >= 0 && j + E <= static_cast<int>(V); }
+  __device__ __forceinline__ bool whole(uint32_t i) const { return i >= lo && i < hi; }
   // position of element j in this block's copy, or -1
   __device__ __forceinline__ int local(int32_t j) const {
     const uint32_t v = (static_cast<uint32_t>(j) + phase) / E;
     return v >= first && v - first < n ? static_cast<int>(static_cast<uint32_t>(j) + phase - first * E) : -1;
   }
+  __device__ __forceinline__ bool starts_on_vector() const { return lo == 0; }
+  // Does f(i) for the (at most two) vectors of this thread that hang over an end.
+  template <class F>
+  __device__ __forceinline__ void ends(F f) const {
+    if (lo && n && threadIdx.x == 0) f(0u);
+    if (hi < n && !(lo && n == 1) && threadIdx.x == (n - 1) % kThreads) f(n - 1);
+  }
   // Starts the copy of this thread's vectors; elements beyond the row's ends become -inf.
   __device__ __forceinline__ void load(uint4* sm) const {
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-      const int j = elem(i);
-      if (whole(j)) {
-        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(sm + i));
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(x + j) : "memory");
-      } else {
-        T* e = reinterpret_cast<T*>(sm + i);
-#pragma unroll
-        for (int q = 0; q < E; ++q)
-          e[q] = j + q >= 0 && j + q < static_cast<int>(V) ? x[j + q] : Ty<T>::from(-INFINITY);
-      }
+    const char* src = reinterpret_cast<const char*>(x) - phase * sizeof(T) + (static_cast<size_t>(first) + threadIdx.x) * 16;
+    uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(sm + threadIdx.x));
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < hi; i += kThreads) {
+      if (i >= lo) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+      src += kThreads * 16;
+      dst += kThreads * 16;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
+    ends([&](uint32_t i) {
+      T* e = reinterpret_cast<T*>(sm + i);
+      const int j = elem(i);
+#pragma unroll
+      for (int q = 0; q < E; ++q) e[q] = j + q >= 0 && j + q < static_cast<int>(V) ? x[j + q] : Ty<T>::from(-INFINITY);
+    });
   }
   static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 };
-
-struct OpMaxNan {      // NaN wins
-  __device__ float operator()(float a, float b) const { return max_nan(a, b); }
-};
-struct OpMax {
-  __device__ double operator()(double a, double b) const { return fmax(a, b); }
-};
-struct OpAdd { template <class V> __device__ V operator()(V a, V b) const { return a + b; } };
-
-// All threads get the result; `scratch` holds kWarps values; the order is fixed.
-template <class V, class Op>
-__device__ __forceinline__ V block_reduce(V v, Op op, V* scratch) {
+template <class T>
+__device__ __forceinline__ void store_elems(T* g, int j, uint32_t V, const float2 (&f)[Ty<T>::E / 2]) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  V r = scratch[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) r = op(r, scratch[w]);
-  return r;
+  for (int q = 0; q < Ty<T>::E; ++q)
+    if (j + q >= 0 && j + q < static_cast<int>(V)) g[j + q] = Ty<T>::from(q & 1 ? f[q / 2].y : f[q / 2].x);
 }
 
-// Softmax statistics of a set of logits: maximum, sum of e = exp((x - max) / T), sum of e * y with
-// y the exponent in powers of two. Sets join by rescaling to the greater maximum.
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+template <class V>
+__device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// ---- softmax statistics --------------------------------------------------------------------------
+// Of a set of logits: maximum m, sum s of e = exp((x - m) / T), sum t of e * y with y the exponent
+// in powers of two. Sets join by rescaling to the greater maximum. A NaN makes all of them NaN, an
+// empty or fully masked set has m = -inf, s = t = 0.
 struct Stats {
   float m, s, t;
 };
@@ -213,34 +222,6 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b, float c) {
   r.t = (a.t + a.s * ya) * ea + (b.t + b.s * yb) * eb;
   return r;
 }
-struct StatsShared {
-  Stats warp[kWarps];
-  Stats block;
-};
-// Statistics of this thread's vectors.
-template <class T, bool ENT>
-__device__ __forceinline__ Stats thread_stats(const uint4* sm, uint32_t n, float m, float c) {
-  const float shift = m == -INFINITY ? 0.0f : m;
-  const float2 sh2 = make_float2(-shift, -shift), c2 = make_float2(c, c);
-  float2 s = make_float2(0.0f, 0.0f), t = make_float2(0.0f, 0.0f);
-#pragma unroll 2
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-    float2 f[Ty<T>::E / 2];
-    Ty<T>::unpack(sm[i], f);
-#pragma unroll
-    for (int q = 0; q < Ty<T>::E / 2; ++q) {
-      float2 y = mul2(add2(f[q], sh2), c2);
-      if (ENT) {                       // a masked token: e = 0 and y must be finite
-        y.x = max_nan(y.x, -200.0f);
-        y.y = max_nan(y.y, -200.0f);
-      }
-      const float2 e = make_float2(ex2(y.x), ex2(y.y));
-      s = add2(s, e);
-      if (ENT) t = fma2(e, y, t);
-    }
-  }
-  return Stats{m, s.x + s.y, t.x + t.y};
-}
 template <class T>
 __device__ __forceinline__ float thread_max(const uint4* sm, uint32_t n) {
   float m = -INFINITY;
@@ -248,115 +229,170 @@ __device__ __forceinline__ float thread_max(const uint4* sm, uint32_t n) {
   for (uint32_t i = threadIdx.x; i < n; i += kThreads) m = max_nan(m, Ty<T>::vmax(sm[i]));
   return m;
 }
-// Statistics of the row, for every thread of every block of the cluster. Contains a cluster barrier:
-// what the blocks wrote to shared memory before it can be read by the others after it.
-__device__ __forceinline__ Stats row_stats(Stats v, float c, StatsShared& sh, cg::cluster_group& cl, uint32_t blocks) {
+template <class T, bool ENT, bool CLAMP>
+__device__ __forceinline__ void thread_sums(const uint4* sm, uint32_t n, float m, float c, float& s_out, float& t_out) {
+  constexpr int H = Ty<T>::E / 2;
+  const float shift = m == -INFINITY ? 0.0f : m;
+  const float2 sh2 = make_float2(-shift, -shift), c2 = make_float2(c, c);
+  float2 s[H], t[H];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
+  for (int q = 0; q < H; ++q) s[q] = t[q] = make_float2(0.0f, 0.0f);
+#pragma unroll 2
+  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+    float2 f[H];
+    Ty<T>::unpack(sm[i], f);
+#pragma unroll
+    for (int q = 0; q < H; ++q) {
+      float2 y = mul2(add2(f[q], sh2), c2);
+      if (CLAMP) {
+        y.x = max_nan(y.x, -200.0f);
+        y.y = max_nan(y.y, -200.0f);
+      }
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      s[q] = add2(s[q], e);
+      if (ENT) t[q] = fma2(e, y, t[q]);
+    }
+  }
+#pragma unroll
+  for (int q = 1; q < H; ++q) { s[0] = add2(s[0], s[q]); t[0] = add2(t[0], t[q]); }
+  s_out = s[0].x + s[0].y;
+  t_out = t[0].x + t[0].y;
+}
+// Statistics of this warp's vectors (the same in all lanes), from its threads' maxima. Only the entropy minds a
+// masked token (0 * -inf): such a warp repeats its sums with the exponents held above -200, where e is 0.
+template <class T, bool ENT>
+__device__ __forceinline__ Stats warp_stats(const uint4* sm, uint32_t n, float tmax, float c) {
+  Stats v;
+  v.m = warp_max_nan(tmax);
+  thread_sums<T, ENT, false>(sm, n, v.m, c, v.s, v.t);
+  if (ENT && __any_sync(0xffffffffu, v.t != v.t)) thread_sums<T, ENT, true>(sm, n, v.m, c, v.s, v.t);
+  v.s = warp_sum(v.s);
+  v.t = ENT ? warp_sum(v.t) : 0.0f;
+  return v;
+}
+struct StatsShared {
+  Stats warp[kWarps];
+  Stats block[kClusterMax];
+};
+// First warp only, after a block barrier behind the writes to sh.warp: this block's statistics, sent to blocks
+// [0, targets) of the cluster. A fixed order: the same bits in every block.
+__device__ __forceinline__ void send_block_stats(StatsShared& sh, float c, cg::cluster_group& cl, uint32_t rank,
+                                                 uint32_t targets) {
+  Stats v = sh.warp[threadIdx.x & (kWarps - 1)];
+#pragma unroll
+  for (int o = kWarps / 2; o > 0; o >>= 1) {
     Stats p;
     p.m = __shfl_xor_sync(0xffffffffu, v.m, o);
     p.s = __shfl_xor_sync(0xffffffffu, v.s, o);
     p.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-    v = (threadIdx.x & o) ? join(p, v, c) : join(v, p, c);      // one order on both sides: the same bits
+    v = (threadIdx.x & o) ? join(p, v, c) : join(v, p, c);
   }
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sh.warp[0];
-  for (int w = 1; w < kWarps; ++w) v = join(v, sh.warp[w], c);
-  if (blocks == 1) return v;
-  if (threadIdx.x == 0) sh.block = v;
-  cl.sync();
-  v = *cl.map_shared_rank(&sh.block, 0);
-  for (uint32_t b = 1; b < blocks; ++b) v = join(v, *cl.map_shared_rank(&sh.block, b), c);
+  if (threadIdx.x < targets) (targets == 1 && rank == 0 ? &sh : cl.map_shared_rank(&sh, threadIdx.x))->block[rank] = v;
+}
+__device__ __forceinline__ Stats row_stats(const StatsShared& sh, float c, uint32_t blocks) {
+  Stats v = sh.block[0];
+  for (uint32_t b = 1; b < blocks; ++b) v = join(v, sh.block[b], c);
   return v;
 }
 
 // ---- token scores ------------------------------------------------------------------------------
 // Order of the alternatives as one integer: greater logit first (-0 equals +0, NaN above all),
 // then the lower index. No two elements of a row share a value; 0 is below all.
+typedef unsigned long long Key;
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return x != x ? 0xffffffffu : (b & 0x80000000u ? ~b : b | 0x80000000u);
 }
-__device__ __forceinline__ unsigned long long rank_key(float x, uint32_t idx) {
-  return (static_cast<unsigned long long>(order_key(x)) << 32) | (0xffffffffu - idx);
+__device__ __forceinline__ Key rank_key(float x, uint32_t idx) {
+  return (static_cast<Key>(order_key(x)) << 32) | (0xffffffffu - idx);
 }
-__device__ __forceinline__ float key_value(unsigned long long key) {
+__device__ __forceinline__ float key_value(Key key) {
   const uint32_t k = static_cast<uint32_t>(key >> 32);
   return k == 0xffffffffu ? nan_f() : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
+constexpr int kCand = 512;                  // candidates of a block's selection
 struct TopShared {
-  unsigned long long cand[kCand];
-  unsigned long long top[kTopMax];
-  uint32_t lo[kWarps], hi[kWarps];
-  uint32_t count;
+  Key cand[kCand];
+  uint32_t key[kThreads];
+  uint16_t hot[kThreads];
+  uint32_t bound, hots, count;
 };
-// Calls f(key) for every element of this thread's vectors whose key is at least `least`.
+// Calls f(key) for the elements of vector i whose value's key is at least `least`.
 template <class T, class F>
-__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4* sm, uint32_t least, F f) {
-  for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
-    const uint4 v = sm[i];
-    if (order_key(Ty<T>::vmax(v)) < least) continue;
-    float2 e[Ty<T>::E / 2];
-    Ty<T>::unpack(v, e);
-    const int j = sh.elem(i);
+__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4* sm, uint32_t i, uint32_t least, F f) {
+  const uint4 v = sm[i];
+  if (order_key(Ty<T>::vmax(v)) < least) return;
+  float2 e[Ty<T>::E / 2];
+  Ty<T>::unpack(v, e);
+  const int j = sh.elem(i);
 #pragma unroll
-    for (int q = 0; q < Ty<T>::E; ++q) {
-      const float x = q & 1 ? e[q / 2].y : e[q / 2].x;
-      if (order_key(x) >= least && j + q >= 0 && j + q < static_cast<int>(sh.V)) f(rank_key(x, j + q));
-    }
+  for (int q = 0; q < Ty<T>::E; ++q) {
+    const float x = q & 1 ? e[q / 2].y : e[q / 2].x;
+    if (order_key(x) >= least && j + q >= 0 && j + q < static_cast<int>(sh.V)) f(rank_key(x, j + q));
   }
 }
-// The best min(k, elements) of this block's share, in order, into ts.top (0 behind the last).
-// Every thread brings the maximum of its vectors: the k-th greatest of those maxima is a bound that at least k
-// elements reach and, since the vectors interleave, few more do. Those few are collected and ranked by counting.
+// The best min(k, elements) of this block's share into out[0..], in order. The caller has put every thread's
+// maximum (order_key, 0 for a thread without data) into ts.key and zeroed ts.hots and ts.count, ahead of a barrier.
+// The k-th greatest of those maxima is a bound that at least k elements reach and, since the threads' vectors
+// interleave, few more do: only the vectors of threads whose maximum reaches it are looked at again, and what
+// they hold is ranked by counting.
 template <class T>
-__device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, float tmax, uint32_t k, TopShared& ts) {
-  const bool have = threadIdx.x < sh.n;
-  const uint32_t key = have ? order_key(tmax) : 0u;
-  {
-    const uint32_t lo = __reduce_min_sync(0xffffffffu, have ? key : 0xffffffffu);
-    const uint32_t hi = __reduce_max_sync(0xffffffffu, key);
-    if ((threadIdx.x & 31) == 0) { ts.lo[threadIdx.x >> 5] = lo; ts.hi[threadIdx.x >> 5] = hi; }
-    if (threadIdx.x == 0) ts.count = 0;
-    for (uint32_t i = threadIdx.x; i < k; i += kThreads) ts.top[i] = 0;
+__device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, uint32_t k, TopShared& ts, Key* out) {
+  constexpr int kPer = kThreads / 32;
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp == 0) {
+    uint32_t bound = 0;                                  // fewer threads than k have data: every element
+    if (sh.n >= k) {
+      uint32_t key[kPer], lo = 0xffffffffu, hi = 0;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        key[q] = ts.key[lane + 32 * q];
+        if (lane + 32 * q < sh.n) lo = min(lo, key[q]);
+        hi = max(hi, key[q]);
+      }
+      lo = __reduce_min_sync(0xffffffffu, lo);           // count(key >= lo) >= k throughout
+      hi = __reduce_max_sync(0xffffffffu, hi);           // nothing to find above
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo) / 2 + 1;
+        uint32_t at = 0;
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) at += key[q] >= mid;
+        at = __reduce_add_sync(0xffffffffu, at);
+        if (at >= k) lo = mid;
+        else hi = mid - 1;
+        if (at >= k && at <= k + k / 4) break;
+      }
+      bound = lo;
+    }
+    if (lane == 0) ts.bound = bound;
   }
   __syncthreads();
-  uint32_t bound = 0;                                    // fewer threads than k have data: every element
-  if (sh.n >= k) {
-    uint32_t lo = 0xffffffffu, hi = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) { lo = min(lo, ts.lo[w]); hi = max(hi, ts.hi[w]); }
-    // count(key >= lo) >= k throughout; above hi nothing is left to find
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo) / 2 + 1;
-      const uint32_t at = __syncthreads_count(key >= mid);
-      if (at >= k) lo = mid;
-      else hi = mid - 1;
-      if (at >= k && at <= k + k / 4) break;
-    }
-    bound = lo;
-  }
-  if (key >= bound && have)
-    each_from(sh, sm, bound, [&](unsigned long long e) {
-      const uint32_t p = atomicAdd(&ts.count, 1u);
-      if (p < kCand) ts.cand[p] = e;
-    });
+  const uint32_t bound = ts.bound;
+  if (threadIdx.x < sh.n && ts.key[threadIdx.x] >= bound) ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
+  __syncthreads();
+  const uint32_t hots = ts.hots;
+  for (uint32_t h = warp; h < hots; h += kWarps)
+    for (uint32_t i = ts.hot[h] + lane * kThreads; i < sh.n; i += 32 * kThreads)
+      each_from(sh, sm, i, bound, [&](Key e) {
+        const uint32_t p = atomicAdd(&ts.count, 1u);
+        if (p < kCand) ts.cand[p] = e;
+      });
   __syncthreads();
   uint32_t found = ts.count;
   if (found > kCand) {
-    // Many equal values or one thread's vectors hold most of the great ones: bisect the (unique) keys of all
-    // elements until exactly k are left.
-    unsigned long long lo = static_cast<unsigned long long>(bound) << 32, hi = ~0ull;
+    // Many equal values, or great ones that share few threads: bisect the (unique) keys of all elements until
+    // exactly k are left.
+    Key lo = static_cast<Key>(bound) << 32, hi = ~0ull;
     while (lo < hi) {
-      const unsigned long long mid = lo + (hi - lo) / 2 + 1;
+      const Key mid = lo + (hi - lo) / 2 + 1;
       uint32_t mine = 0;
-      each_from(sh, sm, static_cast<uint32_t>(mid >> 32), [&](unsigned long long e) { mine += e >= mid; });
+      for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
+        each_from(sh, sm, i, static_cast<uint32_t>(mid >> 32), [&](Key e) { mine += e >= mid; });
       mine = __reduce_add_sync(0xffffffffu, mine);
       __syncthreads();
       if (threadIdx.x == 0) ts.count = 0;
       __syncthreads();
-      if ((threadIdx.x & 31) == 0 && mine) atomicAdd(&ts.count, mine);
+      if (lane == 0 && mine) atomicAdd(&ts.count, mine);
       __syncthreads();
       const uint32_t at = ts.count;
       if (at >= k) lo = mid;
@@ -366,32 +402,53 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, f
     __syncthreads();
     if (threadIdx.x == 0) ts.count = 0;
     __syncthreads();
-    each_from(sh, sm, static_cast<uint32_t>(lo >> 32), [&](unsigned long long e) {
-      if (e >= lo) ts.cand[atomicAdd(&ts.count, 1u)] = e;
-    });
+    for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
+      each_from(sh, sm, i, static_cast<uint32_t>(lo >> 32), [&](Key e) {
+        if (e >= lo) ts.cand[atomicAdd(&ts.count, 1u)] = e;
+      });
     __syncthreads();
     found = ts.count;
   }
   for (uint32_t i = threadIdx.x; i < found; i += kThreads) {
-    const unsigned long long e = ts.cand[i];
+    const Key e = ts.cand[i];
     uint32_t ahead = 0;
+#pragma unroll 4
     for (uint32_t j = 0; j < found; ++j) ahead += ts.cand[j] > e;
-    if (ahead < k) ts.top[ahead] = e;
+    if (ahead < k) out[ahead] = e;
   }
 }
+// Entries of a descending list that are above e.
+__device__ __forceinline__ uint32_t count_above(const Key* list, uint32_t n, Key e) {
+  uint32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (list[mid] > e) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
 
+// Block 0 of a row's cluster writes the results: the others send it their statistics and their own
+// best top_k (behind the row in its shared memory) and leave.
 template <class T, bool ENT>
 __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token_scores d, uint32_t share, uint32_t blocks) {
   extern __shared__ uint4 sm[];
   __shared__ StatsShared ss;
   __shared__ TopShared ts;
   cg::cluster_group cl = cg::this_cluster();
-  const uint32_t rank = blocks == 1 ? 0 : cl.block_rank();
+  const uint32_t rank = blockIdx.x % blocks;           // blocks of a row follow each other, as a cluster's do
   const size_t r = blockIdx.x / blocks;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  Key* lists = reinterpret_cast<Key*>(sm + share);     // [blocks][K]
   const Share<T> sh(d.logits, r, d.row_stride, V, share, rank);
   sh.load(sm);
-  // the given token's logit comes from memory: its block may be any of the cluster's
+  if (K) {
+    if (rank == 0)
+      for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) lists[i] = 0;
+    if (threadIdx.x == 0) ts.hots = ts.count = 0;
+  }
+  if (blocks > 1) cl.barrier_arrive();                 // its wait is where other blocks' memory is first written
+  // the given token's logit comes from memory: it may lie in any block's share
   int32_t lab = -1;
   float xl = 0.0f;
   if (rank == 0 && threadIdx.x == 0 && d.logprob) {
@@ -399,49 +456,48 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
     if (lab >= 0) xl = static_cast<uint32_t>(lab) < V ? Ty<T>::to(sh.x[lab]) : nan_f();
   }
   const float c = kLog2e / d.temperature;
-  sh.wait();                                   // every thread reads only what it copied itself
+  sh.wait();                                           // every thread reads only what it copied itself
   const float tmax = thread_max<T>(sm, sh.n);
-  const Stats mine = thread_stats<T, ENT>(sm, sh.n, tmax, c);
-  if (K) block_top(sh, sm, tmax, K, ts);
-  const Stats row = row_stats(mine, c, ss, cl, blocks);
-  if (rank == 0) {
-    const double S = row.s, logS = log(S), inv_t = 1.0 / static_cast<double>(d.temperature);
-    auto logprob = [&](float x) {
-      return S == 0.0 ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - logS);
-    };
-    if (threadIdx.x == 0) {
-      if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
-      if (d.entropy) d.entropy[r] = S == 0.0 ? 0.0f : static_cast<float>(logS - row.t * kLn2 / S);
-      if (d.stats) {
-        d.stats[2 * r] = row.m;
-        d.stats[2 * r + 1] = row.s;
-      }
-    }
-    if (K) {
-      const unsigned long long* best = ts.top;
-      if (blocks > 1) {                        // join the blocks' lists the same way
-        const uint32_t all = blocks * K;
-        for (uint32_t i = threadIdx.x; i < all; i += kThreads) ts.cand[i] = cl.map_shared_rank(ts.top, i / K)[i % K];
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < all; i += kThreads) {
-          const unsigned long long e = ts.cand[i];
-          if (e == 0) continue;
-          uint32_t ahead = 0;
-          for (uint32_t j = 0; j < all; ++j) ahead += ts.cand[j] > e;
-          if (ahead < K) {
-            d.top_id[r * K + ahead] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
-            d.top_logprob[r * K + ahead] = logprob(key_value(e));
-          }
-        }
-      } else {
-        for (uint32_t i = threadIdx.x; i < K; i += kThreads) {
-          d.top_id[r * K + i] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best[i]));
-          d.top_logprob[r * K + i] = logprob(key_value(best[i]));
-        }
-      }
+  const Stats ws = warp_stats<T, ENT>(sm, sh.n, tmax, c);
+  if ((threadIdx.x & 31) == 0) ss.warp[threadIdx.x >> 5] = ws;
+  if (K) ts.key[threadIdx.x] = threadIdx.x < sh.n ? order_key(tmax) : 0u;
+  __syncthreads();
+  if (blocks > 1) cl.barrier_wait();
+  if (threadIdx.x < 32) send_block_stats(ss, c, cl, rank, 1);
+  if (K) block_top(sh, sm, K, ts, (rank == 0 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
+  if (blocks > 1) {
+    cl.barrier_arrive();
+    if (rank != 0) return;
+    cl.barrier_wait();
+  } else {
+    __syncthreads();
+  }
+  if (threadIdx.x >= blocks * K && threadIdx.x >= 32) return;
+  const Stats row = row_stats(ss, c, blocks);
+  const double S = row.s, logS = log(S), inv_t = 1.0 / static_cast<double>(d.temperature);
+  auto logprob = [&](float x) {
+    return S == 0.0 ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - logS);
+  };
+  if (threadIdx.x == 0) {
+    if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
+    if (d.entropy) d.entropy[r] = S == 0.0 ? 0.0f : static_cast<float>(logS - row.t * kLn2 / S);
+    if (d.stats) {
+      d.stats[2 * r] = row.m;
+      d.stats[2 * r + 1] = row.s;
     }
   }
-  if (blocks > 1) cl.sync();                   // the others' shared memory is read until here
+  for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
+    const Key e = lists[i];
+    if (e == 0) continue;                              // a share of fewer than K elements
+    const uint32_t own = i / K;
+    uint32_t ahead = i - own * K;
+    for (uint32_t b = 0; b < blocks; ++b)
+      if (b != own) ahead += count_above(lists + b * K, K, e);
+    if (ahead < K) {
+      d.top_id[r * K + ahead] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
+      d.top_logprob[r * K + ahead] = logprob(key_value(e));
+    }
+  }
 }
 
 // ---- gradient of the scores ----------------------------------------------------------------------
@@ -449,16 +505,10 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
 // One block per 16 KiB of a row, four vectors in flight per thread.
 constexpr int kGradVecs = 4;
 struct GradRow {
-  float m, a, b, v_label;
+  float m, a, b;
   int32_t label;
   int skip;
 };
-template <class T>
-__device__ __forceinline__ void store_elems(T* g, int j, uint32_t V, const float2 (&f)[Ty<T>::E / 2]) {
-#pragma unroll
-  for (int q = 0; q < Ty<T>::E; ++q)
-    if (j + q >= 0 && j + q < static_cast<int>(V)) g[j + q] = Ty<T>::from(q & 1 ? f[q / 2].y : f[q / 2].x);
-}
 template <class T>
 __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_token_scores_grad d, uint32_t parts) {
   constexpr int E = Ty<T>::E;
@@ -472,32 +522,29 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
     const uint32_t i = threadIdx.x + u * kThreads;
-    if (i < sh.n && sh.whole(sh.elem(i))) v[u] = *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
+    if (sh.whole(i)) v[u] = *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
   }
+  float gl = 0.0f, gh = 0.0f, S = 0.0f, h = 0.0f, xl = 0.0f;
   if (threadIdx.x == 0) {
-    float gl = d.dlogprob ? d.dlogprob[r] : 0.0f;
-    const float gh = d.dentropy ? d.dentropy[r] : 0.0f;
-    const float m = d.stats[2 * r], S = d.stats[2 * r + 1];
+    gl = d.dlogprob ? d.dlogprob[r] : 0.0f;
+    gh = d.dentropy ? d.dentropy[r] : 0.0f;
+    S = d.stats[2 * r + 1];
     int32_t lab = -1;
     if (d.dlogprob) {
       lab = d.labels[r];
       if (lab < 0) gl = 0.0f;
       else if (static_cast<uint32_t>(lab) >= V) { if (gl != 0.0f) gl = nan_f(); lab = -1; }
     }
-    const double inv_t = 1.0 / static_cast<double>(d.temperature);
-    const double logS = log(static_cast<double>(S));
-    const double h = gh != 0.0f ? static_cast<double>(d.entropy[r]) : 0.0;
+    if (gh != 0.0f) h = d.entropy[r];
     gr.skip = (gl == 0.0f && gh == 0.0f) || S == 0.0f;
-    gr.m = m;
-    gr.a = static_cast<float>(inv_t * (-static_cast<double>(gl) - gh * (h - logS)) / S);
-    gr.b = static_cast<float>(inv_t * -static_cast<double>(gh) * kLn2 / S);
+    gr.m = d.stats[2 * r];
+    gr.a = (-gl - gh * (h - logf(S))) / (S * d.temperature);
+    gr.b = -gh * static_cast<float>(kLn2) / (S * d.temperature);
     gr.label = -1;
-    // the label belongs to one block of the row, which reads it before it is overwritten
+    // the label lies in one block's part, which reads it before it is overwritten
     if (lab >= 0 && sh.local(lab) >= 0 && !gr.skip) {
-      const double lp = (static_cast<double>(Ty<T>::to(sh.x[lab])) - m) * inv_t - logS;
-      gr.label = lab;                          // gl (1 - p) without the cancellation, and the entropy's part
-      gr.v_label = static_cast<float>(-static_cast<double>(gl) * inv_t * expm1(lp) +
-                                      (lp == -INFINITY ? 0.0 : -inv_t * gh * exp(lp) * (lp + h)));
+      gr.label = lab;
+      xl = Ty<T>::to(sh.x[lab]);
     }
   }
   __syncthreads();
@@ -511,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
     const uint32_t i = threadIdx.x + u * kThreads;
     if (i >= sh.n) break;
     const int j = sh.elem(i);
-    const bool whole = sh.whole(j);
+    const bool whole = sh.whole(i);
     if (!whole) {
       T* e = reinterpret_cast<T*>(&v[u]);
 #pragma unroll
@@ -532,38 +579,57 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
   }
   if (gr.label >= 0) {
     __syncthreads();
-    if (threadIdx.x == 0) g[gr.label] = Ty<T>::from(gr.v_label);
+    if (threadIdx.x == 0) {                    // gl (1 - p) without the cancellation, and the entropy's part
+      const double inv_t = 1.0 / static_cast<double>(d.temperature);
+      const double lp = (static_cast<double>(xl) - gr.m) * inv_t - log(static_cast<double>(S));
+      const double ent = lp == -INFINITY ? 0.0 : -inv_t * gh * exp(lp) * (lp + h);
+      g[gr.label] = Ty<T>::from(static_cast<float>(-static_cast<double>(gl) * inv_t * expm1(lp) + ent));
+    }
   }
 }
 
 // ---- distillation ------------------------------------------------------------------------------
-// The teacher's side of one row, kept by thread i < top_k for entry i.
+// The teacher's side of one row: thread i < top_k holds entry i, warps without entries skip it. All
+// of it is worked out while the row is on its way to shared memory, in 64 bits: a loss near 0 is a
+// difference of much larger terms.
 struct Entry {
   int32_t id;          // -1: absent (or beyond the list)
   bool first;          // no earlier entry names the token
-  double q, log_q;     // probability of this entry alone
+  float v, x;          // the teacher's value, the student's logit
+  double q, e;         // probability of this entry alone; exp((x - max x) / T) over the entries
 };
+constexpr int kEntryWarps = kTopMax / 32;
 struct TeacherShared {
-  double sd[kWarps];
-  float sf[kWarps];
   __align__(16) int32_t id[kTopMax];
   double q[kTopMax];
-  int bad, dup;
+  double z[kEntryWarps], s[kEntryWarps], l[kEntryWarps];
+  float v[kEntryWarps], x[kEntryWarps];
+  float A, mt;         // of the gradient, once the row is known
+  double named;        // factor of Entry::e in a named token's gradient
+  int bad, dup, empty; // empty: the student's row has no unmasked token
 };
-// Sets rest = q_t; sh.bad when an entry names a token beyond the vocabulary.
-__device__ __forceinline__ void teacher_row(const int32_t* ids, const void* vals, uint32_t vdtype, size_t r, uint32_t K,
-                                            uint32_t V, bool tail, TeacherShared& sh, Entry& e, double& qsum, double& rest) {
+// Entries and the greatest value; a barrier has to follow.
+__device__ __forceinline__ void teacher_load(const int32_t* ids, const void* vals, uint32_t vdtype, size_t r, uint32_t K,
+                                             TeacherShared& sh, Entry& e) {
   const uint32_t i = threadIdx.x;
   e.id = -1;
+  e.v = -INFINITY;
   e.first = false;
-  double v = -INFINITY;
+  if (i >= kTopMax) return;
+  if (i == 0) sh.bad = sh.dup = 0;
   if (i < K) {
     e.id = ids[r * K + i];
-    if (e.id >= 0) v = load_as_f32(vals, vdtype, r * K + i);
+    if (e.id >= 0) e.v = load_as_f32(vals, vdtype, r * K + i);
   }
-  if (i == 0) sh.bad = sh.dup = 0;
-  if (i < kTopMax) sh.id[i] = e.id;
-  __syncthreads();
+  sh.id[i] = e.id;
+  const float top = warp_max_nan(e.v);
+  if ((i & 31) == 0) sh.v[i >> 5] = top;
+}
+// The teacher's exponentials, and which entries are first to name their token; a barrier has to follow.
+__device__ __forceinline__ void teacher_exp(uint32_t V, uint32_t K, bool tail, TeacherShared& sh, Entry& e) {
+  const uint32_t i = threadIdx.x;
+  e.q = 0.0;
+  if ((i & ~31u) >= K) return;
   if (e.id >= 0) {
     if (static_cast<uint32_t>(e.id) >= V) sh.bad = 1;
     uint32_t same = 0;                       // entries before this one that name its token
@@ -575,22 +641,33 @@ __device__ __forceinline__ void teacher_row(const int32_t* ids, const void* vals
     }
     e.first = same == 0;
     if (same) sh.dup = 1;
+    double shift = 0.0;
+    if (!tail) {
+      float vm = sh.v[0];
+      for (uint32_t w = 1; w < kEntryWarps; ++w) vm = max_nan(vm, sh.v[w]);
+      shift = vm == -INFINITY ? 0.0 : vm;
+    }
+    e.q = exp(e.v - shift);
   }
-  if (tail) {
-    e.log_q = v;
-    e.q = exp(v);
-    qsum = block_reduce(e.q, OpAdd(), sh.sd);
-    rest = qsum < 1.0 ? 1.0 - qsum : 0.0;
-  } else {
-    const double vm = block_reduce(v, OpMax(), sh.sd);
-    const double w = vm == -INFINITY ? 0.0 : exp(v - vm);
-    const double z = block_reduce(w, OpAdd(), sh.sd);
-    e.q = z == 0.0 ? 0.0 : w / z;
-    e.log_q = v - vm - log(z);
-    qsum = z == 0.0 ? 0.0 : z != z ? z : 1.0;
-    rest = 0.0;
-  }
-  if (i < K) sh.q[i] = e.q;
+  const double z = warp_sum(e.q);
+  const float x = warp_max_nan(e.x);
+  if ((i & 31) == 0) { sh.z[i >> 5] = z; sh.x[i >> 5] = x; }
+}
+__device__ __forceinline__ double entry_sum(const double* part, uint32_t K) {
+  double s = part[0];
+  for (uint32_t w = 1; 32 * w < K; ++w) s += part[w];
+  return s;
+}
+__device__ __forceinline__ float entry_max(const float* part, uint32_t K) {
+  float m = part[0];
+  for (uint32_t w = 1; 32 * w < K; ++w) m = max_nan(m, part[w]);
+  return m;
+}
+// Sum of the entries' probabilities and the teacher's mass on all other tokens.
+__device__ __forceinline__ void teacher_mass(const TeacherShared& sh, uint32_t K, bool tail, double& qsum, double& rest) {
+  const double z = entry_sum(sh.z, K);
+  qsum = tail ? z : z == 0.0 ? 0.0 : z != z ? z : 1.0;
+  rest = tail && qsum < 1.0 ? 1.0 - qsum : 0.0;
 }
 
 enum Mode { kLoss, kStep, kBackward };
@@ -599,6 +676,21 @@ struct DistillArgs {
   const float* saved_in;       // kBackward
   const float* upstream;       // kBackward: d loss / d row_loss
 };
+
+// Gradient of a row: unnamed tokens get A exp((x - mt) / T) with one factor A for the row, named ones
+// up / T (p Q - q). S is the sum over all tokens at maximum m, st that over the unnamed at mt.
+__device__ __forceinline__ void distill_factors(TeacherShared& th, float up_t, double qsum, double rest, float mt, float st,
+                                                float m, float S, float entry_m, float inv_t) {
+  if (st == 0.0f) rest = 0.0;
+  const float Q = static_cast<float>(qsum + rest);
+  float A = 0.0f;
+  if (st != 0.0f && S != 0.0f) A = up_t * (Q * expf((mt - m) * inv_t) / S - static_cast<float>(rest) / st);
+  if (th.bad || S != S) A = nan_f();
+  th.A = A;
+  th.empty = S == 0.0f;
+  th.mt = mt == -INFINITY ? 0.0f : mt;
+  th.named = S != S ? S : S == 0.0f || entry_m == -INFINITY ? 0.0 : static_cast<double>(Q * expf((entry_m - m) * inv_t) / S);
+}
 
 template <class T, int MODE>
 __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32_t share, uint32_t blocks) {
@@ -611,6 +703,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
   const uint32_t rank = blockIdx.x % blocks;           // blocks of a row follow each other, as a cluster's do
   const size_t r = blockIdx.x / blocks;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  const bool tail = d.tail != 0;
   const Share<T> sh(d.logits, r, d.row_stride, V, share, rank);
   T* g = MODE != kLoss ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
   const bool same = MODE != kLoss && (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
@@ -622,7 +715,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
       for (int q = 0; q < E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
       for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
         const int j = sh.elem(i);
-        if (same && sh.whole(j)) *reinterpret_cast<uint4*>(g + j) = make_uint4(0, 0, 0, 0);
+        if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + j) = make_uint4(0, 0, 0, 0);
         else store_elems<T>(g, j, V, f);
       }
     }
@@ -636,74 +729,122 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
     return;
   }
   sh.load(sm);
-  // the teacher's side, while the row is on its way
+  if (MODE != kBackward && blocks > 1) cl.barrier_arrive();    // waited for ahead of the first write to another block
   Entry e;
-  double qsum, rest;
-  teacher_row(d.teacher_id, d.teacher_logprob, d.teacher_dtype, r, K, V, d.tail != 0, th, e, qsum, rest);
-  const bool bad = th.bad != 0;
-  const int at = e.id >= 0 && !bad ? sh.local(e.id) : -1;
-  float xe = -INFINITY;
-  if (MODE != kBackward && e.id >= 0 && !bad) xe = Ty<T>::to(sh.x[e.id]);
-  const float c = kLog2e / d.temperature;
-  const double inv_t = 1.0 / static_cast<double>(d.temperature);
+  teacher_load(d.teacher_id, d.teacher_logprob, d.teacher_dtype, r, K, th, e);
+  e.x = -INFINITY;
+  // read here, ahead of the cluster's barrier: in place, another block may overwrite it behind that
+  if (MODE != kBackward && e.id >= 0 && static_cast<uint32_t>(e.id) < V) e.x = Ty<T>::to(sh.x[e.id]);
+  __syncthreads();
+  teacher_exp(V, K, tail, th, e);
+  const float c = kLog2e / d.temperature, inv_t = 1.0f / d.temperature;
   sh.wait();
   __syncthreads();
   // named tokens leave the parked row: what is left is the student's tail, summed without a difference
-  if (MODE == kBackward && at >= 0) xe = Ty<T>::to(reinterpret_cast<T*>(sm)[at]);
-  __syncthreads();
+  const bool bad = th.bad != 0;
+  const int at = e.id >= 0 && !bad ? sh.local(e.id) : -1;
+  e.e = 0.0;
+  float entry_m = -INFINITY;
+  if ((threadIdx.x & ~31u) < K) {
+    if (MODE == kBackward) {
+      entry_m = 0.0f;                                  // Entry::e is taken against the row's maximum below
+      if (at >= 0) e.x = Ty<T>::to(reinterpret_cast<T*>(sm)[at]);
+      __syncwarp();
+    } else {
+      entry_m = entry_max(th.x, K);
+    }
+    if (!tail) {
+      const double z = entry_sum(th.z, K);
+      e.q = z == 0.0 ? 0.0 : e.q / z;
+    }
+    th.q[threadIdx.x] = e.q;
+  }
+  if (MODE == kBackward) __syncthreads();              // two entries may name one token: both have read it
   if (at >= 0) reinterpret_cast<T*>(sm)[at] = Ty<T>::from(-INFINITY);
+  if (MODE != kBackward && (threadIdx.x & ~31u) < K) {
+    const double t64 = 1.0 / static_cast<double>(d.temperature);
+    const double y = (static_cast<double>(e.x) - entry_m) * t64;
+    if (e.first && !bad && e.x != -INFINITY) e.e = exp(y);
+    double l = 0.0;                                    // sum of q (ln q - (x - max) / T)
+    if (e.q != 0.0) {
+      const double log_q = tail ? e.v : e.v - static_cast<double>(entry_max(th.v, K)) - log(entry_sum(th.z, K));
+      l = e.x == -INFINITY ? INFINITY : e.q * (log_q - y);
+    }
+    const double s = warp_sum(e.e);
+    l = warp_sum(l);
+    if ((threadIdx.x & 31) == 0) { th.s[threadIdx.x >> 5] = s; th.l[threadIdx.x >> 5] = l; }
+  }
   __syncthreads();
-  float mt, m;
-  double st, S;
+  double qsum, rest;
+  const float up_t = (MODE == kBackward ? 1.0f : d.scale) * w * inv_t;
   if (MODE != kBackward) {
     const float tmax = thread_max<T>(sm, sh.n);
-    const Stats row = row_stats(thread_stats<T, false>(sm, sh.n, tmax, c), c, ss, cl, blocks);
-    mt = row.m;
-    st = row.s;
-    m = max_nan(mt, block_reduce(xe, OpMaxNan(), th.sf));
-    S = block_reduce(e.first && !bad && xe != -INFINITY ? exp((static_cast<double>(xe) - m) * inv_t) : 0.0, OpAdd(), th.sd);
-    if (st != 0.0) S += st * exp((static_cast<double>(mt) - m) * inv_t);
-    if (st != st || m != m) S = nan_f();
-    if (rank == 0) {
-      const double logS = log(S);
-      double l = 0.0;
-      if (e.q != 0.0 && e.id >= 0) l = S == 0.0 ? INFINITY : e.q * (e.log_q - ((static_cast<double>(xe) - m) * inv_t - logS));
-      l = block_reduce(l, OpAdd(), th.sd);
-      if (rest > 0.0 && st != 0.0) l += rest * (log(rest) - ((static_cast<double>(mt) - m) * inv_t + log(st) - logS));
+    const Stats ws = warp_stats<T, false>(sm, sh.n, tmax, c);
+    if ((threadIdx.x & 31) == 0) ss.warp[threadIdx.x >> 5] = ws;
+    __syncthreads();
+    if (blocks > 1) cl.barrier_wait();
+    if (threadIdx.x < 32) send_block_stats(ss, c, cl, rank, MODE == kLoss ? 1 : blocks);
+    if (blocks > 1) {
+      cl.barrier_arrive();
+      if (MODE == kLoss && rank != 0) return;
+      cl.barrier_wait();
+    } else {
+      __syncthreads();
+    }
+    if (MODE == kStep) {
       if (threadIdx.x == 0) {
-        d.row_loss[r] = bad ? nan_f() : static_cast<float>(l);
-        if (d.saved) {
-          float* sv = d.saved + 4 * r;
-          sv[0] = mt; sv[1] = static_cast<float>(st); sv[2] = m; sv[3] = static_cast<float>(S);
-        }
+        const Stats row = row_stats(ss, c, blocks);
+        const float m = max_nan(row.m, entry_m);
+        float S = 0.0f;
+        if (row.s != 0.0f) S = row.s * expf((row.m - m) * inv_t);
+        const float es = static_cast<float>(entry_sum(th.s, K));
+        if (es != 0.0f) S += es * expf((entry_m - m) * inv_t);
+        if (m != m) S = nan_f();
+        teacher_mass(th, K, tail, qsum, rest);
+        distill_factors(th, up_t, qsum, rest, row.m, row.s, m, S, entry_m, inv_t);
       }
+      __syncthreads();
     }
   } else {
     const float* sv = a.saved_in + 4 * r;
-    mt = sv[0]; st = sv[1]; m = sv[2]; S = sv[3];
+    const float m = sv[2];
+    if (at >= 0 && e.x != -INFINITY) e.e = exp((static_cast<double>(e.x) - m) / d.temperature);
+    if (threadIdx.x == 0) {
+      teacher_mass(th, K, tail, qsum, rest);
+      distill_factors(th, up_t, qsum, rest, sv[0], sv[1], m, sv[3], m, inv_t);
+    }
+    __syncthreads();
   }
   if (MODE != kLoss) {
-    // unnamed tokens: A exp((x - mt) / T); named ones: (p Q - q) up / T
-    const double up = (MODE == kBackward ? 1.0 : static_cast<double>(d.scale)) * w * inv_t;
-    if (st == 0.0) rest = 0.0;
-    const double Q = qsum + rest;
-    double A = 0.0;
-    if (st != 0.0 && S != 0.0) A = up * (Q * exp((static_cast<double>(mt) - m) * inv_t) / S - rest / st);
-    if (bad || S != S) A = nan_f();
-    const float sf = mt == -INFINITY ? 0.0f : -mt;
-    const float2 shift = make_float2(sf, sf), c2 = make_float2(c, c);
-    const float2 A2 = make_float2(static_cast<float>(A), static_cast<float>(A));
-    for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
-      const int j = sh.elem(i);
-      float2 f[E / 2];
+    const float2 shift = make_float2(-th.mt, -th.mt), c2 = make_float2(c, c), A2 = make_float2(th.A, th.A);
+    auto grad = [&](uint32_t i, float2 (&f)[E / 2]) {
       Ty<T>::unpack(sm[i], f);
 #pragma unroll
       for (int q = 0; q < E / 2; ++q) {
         const float2 y = mul2(add2(f[q], shift), c2);
         f[q] = mul2(make_float2(ex2(y.x), ex2(y.y)), A2);
       }
-      if (same && sh.whole(j)) *reinterpret_cast<uint4*>(g + j) = Ty<T>::pack(f);
-      else store_elems<T>(g, j, V, f);
+    };
+    if (same) {
+      T* dst = g + sh.elem(threadIdx.x);
+#pragma unroll 2
+      for (uint32_t i = threadIdx.x; i < sh.hi; i += kThreads) {
+        float2 f[E / 2];
+        grad(i, f);
+        if (i >= sh.lo) *reinterpret_cast<uint4*>(dst) = Ty<T>::pack(f);
+        dst += kThreads * E;
+      }
+      sh.ends([&](uint32_t i) {
+        float2 f[E / 2];
+        grad(i, f);
+        store_elems<T>(g, sh.elem(i), V, f);
+      });
+    } else {
+      for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
+        float2 f[E / 2];
+        grad(i, f);
+        store_elems<T>(g, sh.elem(i), V, f);
+      }
     }
     __syncthreads();
     if (at >= 0 && e.first) {
@@ -713,24 +854,50 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
         for (uint32_t j = 0; j < K; ++j)
           if (th.id[j] == e.id) q += th.q[j];
       }
-      const double p = S == 0.0 ? 0.0 : exp((static_cast<double>(xe) - m) * inv_t) / S;
-      g[e.id] = Ty<T>::from(S == 0.0 ? 0.0f : static_cast<float>(up * (p * Q - q)));
+      g[e.id] = Ty<T>::from(th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named - q)));
     }
   }
-  if (MODE != kBackward && blocks > 1) cl.sync();      // the others' shared memory is read until here
+  if (MODE != kBackward && rank == 0 && threadIdx.x == 0) {
+    const Stats row = row_stats(ss, c, blocks);
+    const double t64 = 1.0 / static_cast<double>(d.temperature), st = row.s, es = entry_sum(th.s, K);
+    const float m = max_nan(row.m, entry_m);
+    double S = 0.0;
+    if (st != 0.0) S = st * exp((static_cast<double>(row.m) - m) * t64);
+    if (es != 0.0) S += es * exp((static_cast<double>(entry_m) - m) * t64);
+    if (m != m) S = nan_f();
+    teacher_mass(th, K, tail, qsum, rest);
+    const double logS = log(S);
+    double l = entry_sum(th.l, K);
+    if (qsum != 0.0) l += qsum * ((static_cast<double>(m) - entry_m) * t64 + logS);
+    if (qsum != 0.0 && S == 0.0) l = INFINITY;
+    if (rest > 0.0 && st != 0.0) l += rest * (log(rest) - ((static_cast<double>(row.m) - m) * t64 + log(st) - logS));
+    d.row_loss[r] = bad ? nan_f() : static_cast<float>(l);
+    if (d.saved) {
+      float* sv = d.saved + 4 * r;
+      sv[0] = row.m; sv[1] = row.s; sv[2] = m; sv[3] = static_cast<float>(S);
+    }
+  }
 }
 
-__global__ void __launch_bounds__(kThreads) row_loss_sum_kernel(const float* __restrict__ row_loss,
-                                                                const float* __restrict__ weight, size_t rows, float scale,
-                                                                float* __restrict__ loss) {
-  __shared__ double sd[kWarps];
+// loss = scale * sum of weight * row_loss, in a fixed order and 64 bits: one block, four rows in flight per thread.
+constexpr int kSumThreads = 1024;
+__global__ void __launch_bounds__(kSumThreads) row_loss_sum_kernel(const float* __restrict__ row_loss,
+                                                                   const float* __restrict__ weight, size_t rows, float scale,
+                                                                   float* __restrict__ loss) {
+  __shared__ double part[kSumThreads / 32];
   double s = 0.0;
-  for (size_t r = threadIdx.x; r < rows; r += kThreads) {
-    const double w = weight ? weight[r] : 1.0f;
-    if (w != 0.0) s += w * row_loss[r];
+#pragma unroll 4
+  for (size_t r = threadIdx.x; r < rows; r += kSumThreads) {
+    const float w = weight ? weight[r] : 1.0f, l = row_loss[r];
+    if (w != 0.0f) s += static_cast<double>(w) * l;
   }
-  s = block_reduce(s, OpAdd(), sd);
-  if (threadIdx.x == 0) *loss = static_cast<float>(s * scale);
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(part[threadIdx.x]);
+    if (threadIdx.x == 0) *loss = static_cast<float>(s * scale);
+  }
 }
 
 // ---- launches ------------------------------------------------------------------------------------
@@ -740,7 +907,7 @@ int by_type(uint32_t dtype, F f) {
   if (dtype == SEEML_B200_DTYPE_BF16) return f(__nv_bfloat16{});
   return f(__half{});
 }
-// Blocks per row. A share of at most 72 KiB lets three blocks live on an SM, so that one copies
+// Blocks per row. A share of at most 66 KiB lets three blocks live on an SM, so that one copies
 // while others compute; a call of few rows is spread further, down to 8 KiB a block, until it
 // covers the SMs.
 struct Split {
@@ -749,11 +916,11 @@ struct Split {
 Split split_row(uint64_t rows, uint64_t vocab, uint64_t elem) {
   const uint64_t per = 16 / elem, vecs = (vocab + 2 * (per - 1)) / per;    // whatever the row's phase
   uint64_t blocks = 1;
-  while (blocks < kClusterMax && vecs * 16 > blocks * (72u << 10)) blocks *= 2;
+  while (blocks < kClusterMax && vecs * 16 > blocks * (66u << 10)) blocks *= 2;
   while (blocks < kClusterMax && rows * blocks < kSMs && vecs * 16 > blocks * (8u << 10)) blocks *= 2;
   return {static_cast<uint32_t>(blocks), static_cast<uint32_t>((vecs + blocks - 1) / blocks)};
 }
-constexpr uint32_t kMaxDynamic = 200u << 10;
+constexpr uint32_t kMaxDynamic = 208u << 10;    // 192 KiB of a row and eight lists of alternatives
 // Allows the kernel its shared memory, once per device (many threads may do it at the same time).
 template <class Kernel>
 bool allow_smem(Kernel kernel, std::atomic<uint64_t>& done) {
@@ -766,13 +933,13 @@ bool allow_smem(Kernel kernel, std::atomic<uint64_t>& done) {
   return true;
 }
 template <auto Kernel, class... Args>
-int launch_rows(uint64_t rows, const Split& s, bool cluster, cudaStream_t st, Args... args) {
+int launch_rows(uint64_t rows, const Split& s, bool cluster, size_t lists, cudaStream_t st, Args... args) {
   static std::atomic<uint64_t> done{0};
   if (!allow_smem(Kernel, done)) return -1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * s.blocks));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = s.share * 16;
+  cfg.dynamicSmemBytes = s.share * 16 + lists;
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
@@ -790,8 +957,9 @@ int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
   const Split s = split_row(d.rows, d.vocab, elem_bytes(d.dtype));
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
-    return d.entropy ? launch_rows<token_scores_kernel<T, true>>(d.rows, s, true, st, d)
-                     : launch_rows<token_scores_kernel<T, false>>(d.rows, s, true, st, d);
+    const size_t lists = sizeof(Key) * s.blocks * d.top_k;
+    return d.entropy ? launch_rows<token_scores_kernel<T, true>>(d.rows, s, true, lists, st, d)
+                     : launch_rows<token_scores_kernel<T, false>>(d.rows, s, true, lists, st, d);
   });
 }
 int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st) {
@@ -809,8 +977,8 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
   const DistillArgs a{d, nullptr, nullptr};
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
-    return d.dlogits ? launch_rows<distill_kernel<T, kStep>>(d.rows, s, true, st, a)
-                     : launch_rows<distill_kernel<T, kLoss>>(d.rows, s, true, st, a);
+    return d.dlogits ? launch_rows<distill_kernel<T, kStep>>(d.rows, s, true, 0, st, a)
+                     : launch_rows<distill_kernel<T, kLoss>>(d.rows, s, true, 0, st, a);
   });
 }
 int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
@@ -833,11 +1001,11 @@ int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
   a.upstream = b.drow_loss;
   return by_type(b.dtype, [&](auto t) {
     using T = decltype(t);
-    return launch_rows<distill_kernel<T, kBackward>>(b.rows, s, false, st, a);
+    return launch_rows<distill_kernel<T, kBackward>>(b.rows, s, false, 0, st, a);
   });
 }
 int row_loss_sum(const float* row_loss, const float* weight, size_t rows, float scale, float* loss, cudaStream_t st) {
-  row_loss_sum_kernel<<<1, kThreads, 0, st>>>(row_loss, weight, rows, scale, loss);
+  row_loss_sum_kernel<<<1, kSumThreads, 0, st>>>(row_loss, weight, rows, scale, loss);
   return 1;
 }
 

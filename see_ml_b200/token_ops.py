@@ -28,7 +28,7 @@ _F32, _I32 = torch.float32, torch.int32
 class TokenScores(NamedTuple):
     logprob: Optional[torch.Tensor]      # [rows] f32, None without labels
     entropy: Optional[torch.Tensor]      # [rows] f32
-    stats: torch.Tensor                  # [rows, 2] f32: max, sum exp((x - max) / T)
+    stats: Optional[torch.Tensor]        # [rows, 2] f32: max, sum exp((x - max) / T); for token_scores_backward
     top_logprob: Optional[torch.Tensor]  # [rows, top_k] f32
     top_id: Optional[torch.Tensor]       # [rows, top_k] i32
 
@@ -86,7 +86,7 @@ def _gradient(logits, out):
 
 
 def _call(fn, desc, device):
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream() without building its object
     if torch.cuda.current_device() == device.index:
         rc = fn(C.byref(desc), stream)
     else:
@@ -96,7 +96,7 @@ def _call(fn, desc, device):
         raise L.BackendError(L.last_error())
 
 
-def token_scores(logits, labels=None, *, top_k=0, temperature=1.0, entropy=True) -> TokenScores:
+def token_scores(logits, labels=None, *, top_k=0, temperature=1.0, entropy=True, stats=False) -> TokenScores:
     """Log probability of `labels` (i32, negative = none), entropy and the `top_k` alternatives."""
     _matrix("logits", logits)
     rows, vocab = logits.shape
@@ -106,15 +106,15 @@ def token_scores(logits, labels=None, *, top_k=0, temperature=1.0, entropy=True)
     lab = _operand("labels", labels, (rows,), (_I32,), dev)
     logprob = torch.empty(rows, dtype=_F32, device=dev) if labels is not None else None
     ent = torch.empty(rows, dtype=_F32, device=dev) if entropy else None
-    stats = torch.empty((rows, 2), dtype=_F32, device=dev)
+    st = torch.empty((rows, 2), dtype=_F32, device=dev) if stats else None
     top_lp = torch.empty((rows, top_k), dtype=_F32, device=dev) if top_k else None
     top_id = torch.empty((rows, top_k), dtype=_I32, device=dev) if top_k else None
     d = L.TokenScores(logits.data_ptr(), lab, logprob.data_ptr() if logprob is not None else None,
-                      ent.data_ptr() if entropy else None, stats.data_ptr(), top_lp.data_ptr() if top_k else None,
+                      ent.data_ptr() if entropy else None, st.data_ptr() if stats else None, top_lp.data_ptr() if top_k else None,
                       top_id.data_ptr() if top_k else None, rows, vocab, _stride(logits), _DTYPES[logits.dtype], top_k,
                       temperature, 0)
     _call(L.lib().seeml_b200_token_scores_fwd, d, dev)
-    return TokenScores(logprob, ent, stats, top_lp, top_id)
+    return TokenScores(logprob, ent, st, top_lp, top_id)
 
 
 def token_scores_backward(logits, labels, stats, entropy, dlogprob, dentropy, *, temperature=1.0, out=None):

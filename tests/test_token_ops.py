@@ -151,7 +151,7 @@ def test_token_scores(backend_lib, rows, V, dtype, pad, T, masked, k):
     rng = np.random.default_rng(V * 31 + k)
     _, x = _logits(rng, rows, V, dtype, pad, masked=masked)
     labels = rng.integers(-1, V, rows).astype(np.int32)
-    s = ops.token_scores(x, torch.from_numpy(labels).cuda(), top_k=k, temperature=T)
+    s = ops.token_scores(x, torch.from_numpy(labels).cuda(), top_k=k, temperature=T, stats=True)
     lp, h, tlp, tid = R.scores(_f64(x), labels, k, T)
     d = R.delta(V)
     _close(s.logprob, lp, d, F32, "logprob")
@@ -196,7 +196,7 @@ def test_rows_that_are_masked_or_not_finite(backend_lib, V):
     x[5, 4] = np.nan
     t = torch.from_numpy(x).float().cuda()
     labels = np.array([1, 0, 0, 0, 1, 3, V + 5], np.int32)
-    s = ops.token_scores(t, torch.from_numpy(labels).cuda(), top_k=4, temperature=0.5)
+    s = ops.token_scores(t, torch.from_numpy(labels).cuda(), top_k=4, temperature=0.5, stats=True)
     lp, h, tlp, tid = R.scores(_f64(t), labels, 4, 0.5)
     np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
     _close(s.logprob, lp, R.delta(V), F32, "logprob")
@@ -219,7 +219,7 @@ def test_token_scores_gradient(backend_lib, rows, V, dtype, pad, T, masked, part
     gl, gh = rng.standard_normal((2, rows)).astype(np.float32)
     gl[rows // 2] = gh[rows // 2] = 0.0
     lab = torch.from_numpy(labels).cuda()
-    s = ops.token_scores(x, lab, temperature=T)
+    s = ops.token_scores(x, lab, temperature=T, stats=True)
     up = [torch.from_numpy(v).cuda() for v in (gl, gh)]
     g = ops.token_scores_backward(x, lab, s.stats, s.entropy, up[0] if parts != "entropy" else None,
                                   up[1] if parts != "logprob" else None, temperature=T)
@@ -330,7 +330,7 @@ def test_gradients_against_differences(backend_lib, tail):
     r = ops.distill_topk(x, ids, v, temperature=T, tail=tail, grad=True)
     f = ops.distill_topk(steps, ids.expand(2 * V, -1).contiguous(), v.expand(2 * V, -1).contiguous(), temperature=T, tail=tail).row_loss
     lab = torch.tensor([4], dtype=torch.int32, device="cuda")
-    s = ops.token_scores(x, lab, temperature=T)
+    s = ops.token_scores(x, lab, temperature=T, stats=True)
     one = torch.ones(1, device="cuda")
     g = ops.token_scores_backward(x, lab, s.stats, s.entropy, one, -one, temperature=T)
     f2 = ops.token_scores(steps, lab.expand(2 * V).contiguous(), temperature=T)
@@ -357,7 +357,7 @@ def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs):
     lab = torch.zeros(rows, dtype=torch.int32, device="cuda")
     one = torch.ones(rows, device="cuda")
     flat = x.contiguous()
-    s0, s1 = ops.token_scores(flat, lab, top_k=9), ops.token_scores(x, lab, top_k=9)
+    s0, s1 = ops.token_scores(flat, lab, top_k=9), ops.token_scores(x, lab, top_k=9, stats=True)
     assert torch.equal(s0.top_id, s1.top_id)
     _close(s1.logprob, _f64(s0.logprob), 2 * R.delta(V), F32, "logprob")
     loss, lerr, grad, gerr = R.distill(_f64(x), ids.cpu().numpy(), _f64(v), 1.0, True)
@@ -440,7 +440,7 @@ def test_streams_and_graphs_give_the_same_bits(backend_lib):
     one = torch.ones(rows, device="cuda")
 
     def step(teacher, student):
-        s = ops.token_scores(teacher, lab, top_k=k)
+        s = ops.token_scores(teacher, lab, top_k=k, stats=True)
         r = ops.distill_topk(student, s.top_id, s.top_logprob, scale=1 / rows, tail=True, grad=True)
         g = ops.token_scores_backward(teacher, lab, s.stats, s.entropy, one, -one)
         return [s.logprob, s.entropy, s.top_id, s.top_logprob, r.loss, r.row_loss, r.dlogits, g]
