@@ -133,20 +133,20 @@ __device__ __forceinline__ float load_as_f32(const void* p, uint32_t dtype, size
 
 // ---- one block's share of a row ------------------------------------------------------------------
 // The row is cut into the 16-byte vectors of its memory: vector v holds elements v*E - phase ...
-// +E-1, the first and the last may hang over the row's ends. Block `rank` of the row owns vectors
-// [rank*share, rank*share + n); thread t owns its vectors t, t + kThreads, ... Vectors [lo, hi) of
-// the share lie inside the row as a whole.
+// +E-1, the first and the last may hang over the row's ends. The row's blocks own n vectors each
+// (within one), in order; thread t of a block owns the block's vectors t, t + kThreads, ...
+// Vectors [lo, hi) of the share lie inside the row as a whole.
 template <class T>
 struct Share {
   static constexpr int E = Ty<T>::E;
   const T* x;            // the row
   uint32_t V, phase, first, n, lo, hi;
-  __device__ __forceinline__ Share(const void* base, size_t row, size_t stride, uint32_t V_, uint32_t share, uint32_t rank)
+  __device__ __forceinline__ Share(const void* base, size_t row, size_t stride, uint32_t V_, uint32_t blocks, uint32_t rank)
       : x(static_cast<const T*>(base) + row * stride), V(V_) {
     phase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T);
     const uint32_t nvec = (V + phase + E - 1) / E;
-    first = rank * share;
-    n = nvec <= first ? 0u : (nvec - first < share ? nvec - first : share);
+    first = nvec * rank / blocks;                // a row has at most 2^17 vectors
+    n = nvec * (rank + 1) / blocks - first;
     lo = first == 0 && phase ? 1u : 0u;
     hi = n && (first + n) * E - phase > V ? n - 1 : n;
   }
@@ -258,41 +258,63 @@ __device__ __forceinline__ void thread_sums(const uint4* sm, uint32_t n, float m
   s_out = s[0].x + s[0].y;
   t_out = t[0].x + t[0].y;
 }
-// Statistics of this warp's vectors (the same in all lanes), from its threads' maxima. Only the entropy minds a
-// masked token (0 * -inf): such a warp repeats its sums with the exponents held above -200, where e is 0.
+// Sums of this warp's vectors (the same in all lanes) against the maximum m. Only the entropy minds a masked token
+// (0 * -inf): such a warp repeats its sums with the exponents held above -200, where e is 0.
 template <class T, bool ENT>
-__device__ __forceinline__ Stats warp_stats(const uint4* sm, uint32_t n, float tmax, float c) {
-  Stats v;
-  v.m = warp_max_nan(tmax);
-  thread_sums<T, ENT, false>(sm, n, v.m, c, v.s, v.t);
-  if (ENT && __any_sync(0xffffffffu, v.t != v.t)) thread_sums<T, ENT, true>(sm, n, v.m, c, v.s, v.t);
-  v.s = warp_sum(v.s);
-  v.t = ENT ? warp_sum(v.t) : 0.0f;
-  return v;
+__device__ __forceinline__ void warp_sums(const uint4* sm, uint32_t n, float m, float c, float& s, float& t) {
+  thread_sums<T, ENT, false>(sm, n, m, c, s, t);
+  if (ENT && __any_sync(0xffffffffu, t != t)) thread_sums<T, ENT, true>(sm, n, m, c, s, t);
+  s = warp_sum(s);
+  t = ENT ? warp_sum(t) : 0.0f;
 }
 struct StatsShared {
-  Stats warp[kWarps];
+  __align__(16) float m[kWarps];
+  float s[kWarps], t[kWarps];
   Stats block[kClusterMax];
 };
-// First warp only, after a block barrier behind the writes to sh.warp: this block's statistics, sent to blocks
-// [0, targets) of the cluster. A fixed order: the same bits in every block.
-__device__ __forceinline__ void send_block_stats(StatsShared& sh, float c, cg::cluster_group& cl, uint32_t rank,
-                                                 uint32_t targets) {
-  Stats v = sh.warp[threadIdx.x & (kWarps - 1)];
+__device__ __forceinline__ float block_max(const StatsShared& sh) {
+  float m = sh.m[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) m = max_nan(m, sh.m[w]);
+  return m;
+}
+// First warp only, after a block barrier behind the writes to sh.s and sh.t: this block's statistics, sent to blocks
+// [0, targets) of the cluster (the block alone when it is one). A fixed order: the same bits in every run.
+__device__ __forceinline__ void send_block_stats(StatsShared& sh, float m, cg::cluster_group& cl, uint32_t rank,
+                                                 uint32_t blocks, uint32_t targets) {
+  Stats v;
+  v.m = m;
+  v.s = sh.s[threadIdx.x & (kWarps - 1)];
+  v.t = sh.t[threadIdx.x & (kWarps - 1)];
 #pragma unroll
   for (int o = kWarps / 2; o > 0; o >>= 1) {
-    Stats p;
-    p.m = __shfl_xor_sync(0xffffffffu, v.m, o);
-    p.s = __shfl_xor_sync(0xffffffffu, v.s, o);
-    p.t = __shfl_xor_sync(0xffffffffu, v.t, o);
-    v = (threadIdx.x & o) ? join(p, v, c) : join(v, p, c);
+    v.s += __shfl_xor_sync(0xffffffffu, v.s, o);
+    v.t += __shfl_xor_sync(0xffffffffu, v.t, o);
   }
-  if (threadIdx.x < targets) (targets == 1 && rank == 0 ? &sh : cl.map_shared_rank(&sh, threadIdx.x))->block[rank] = v;
+  if (threadIdx.x < targets) (blocks == 1 ? &sh : cl.map_shared_rank(&sh, threadIdx.x))->block[rank] = v;
 }
 __device__ __forceinline__ Stats row_stats(const StatsShared& sh, float c, uint32_t blocks) {
   Stats v = sh.block[0];
   for (uint32_t b = 1; b < blocks; ++b) v = join(v, sh.block[b], c);
   return v;
+}
+// The cluster's barrier, arrival and wait apart. Only a warp that wrote to another block's memory has to make that
+// visible; for the others the arrival costs no fence.
+__device__ __forceinline__ void cluster_arrive(bool wrote) {
+  if (wrote) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  else asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// ln S of an exponential sum: 1 <= S (its greatest term is 1), 0 for a row without terms, or NaN. The mantissa's
+// logarithm is below 0.35 in magnitude, so its f32 error is too small to matter beside an exponent summed in 64 bits.
+__device__ __forceinline__ double ln_sum(float S) {
+  if (!(S > 0.0f)) return S == 0.0f ? -INFINITY : static_cast<double>(S);
+  const uint32_t b = __float_as_uint(S);
+  int e = static_cast<int>(b >> 23) - 127;
+  float f = __uint_as_float((b & 0x007fffffu) | 0x3f800000u);
+  if (f > 1.41421356f) { f *= 0.5f; ++e; }
+  return e * kLn2 + static_cast<double>(logf(f));
 }
 
 // ---- token scores ------------------------------------------------------------------------------
@@ -312,71 +334,76 @@ __device__ __forceinline__ float key_value(Key key) {
 }
 constexpr int kCand = 512;                  // candidates of a block's selection
 struct TopShared {
-  Key cand[kCand];
+  __align__(16) Key cand[kCand];
   uint32_t key[kThreads];
   uint16_t hot[kThreads];
-  uint32_t bound, hots, count;
+  uint32_t bound[kClusterMax], hots, count;
 };
-// Calls f(key) for the elements of vector i whose value's key is at least `least`.
+// Calls f(key) for the elements of vector i whose key is at least `least` (thr: the value of that key).
 template <class T, class F>
-__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4* sm, uint32_t i, uint32_t least, F f) {
-  const uint4 v = sm[i];
-  if (order_key(Ty<T>::vmax(v)) < least) return;
+__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4* sm, uint32_t i, uint32_t least, float thr, F f) {
   float2 e[Ty<T>::E / 2];
-  Ty<T>::unpack(v, e);
-  const int j = sh.elem(i);
+  Ty<T>::unpack(sm[i], e);
+  uint32_t hit = 0;
 #pragma unroll
-  for (int q = 0; q < Ty<T>::E; ++q) {
-    const float x = q & 1 ? e[q / 2].y : e[q / 2].x;
+  for (int q = 0; q < Ty<T>::E; ++q)
+    if (!((q & 1 ? e[q / 2].y : e[q / 2].x) < thr)) hit |= 1u << q;        // NaN passes
+  const int j = sh.elem(i);
+  const T* v = reinterpret_cast<const T*>(sm + i);
+  while (hit) {
+    const int q = __ffs(hit) - 1;
+    hit &= hit - 1;
+    const float x = Ty<T>::to(v[q]);
     if (order_key(x) >= least && j + q >= 0 && j + q < static_cast<int>(sh.V)) f(rank_key(x, j + q));
   }
 }
-// The best min(k, elements) of this block's share into out[0..], in order. The caller has put every thread's
-// maximum (order_key, 0 for a thread without data) into ts.key and zeroed ts.hots and ts.count, ahead of a barrier.
-// The k-th greatest of those maxima is a bound that at least k elements reach and, since the threads' vectors
-// interleave, few more do: only the vectors of threads whose maximum reaches it are looked at again, and what
-// they hold is ranked by counting.
-template <class T>
-__device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, uint32_t k, TopShared& ts, Key* out) {
+// A bound that at least k of the block's elements reach: the k-th greatest of its threads' maxima, or a lower one that
+// at most half as many again reach. First warp only; 0 (every element) when fewer threads than k have data.
+__device__ __forceinline__ uint32_t top_bound(const TopShared& ts, uint32_t n, uint32_t k) {
   constexpr int kPer = kThreads / 32;
-  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp == 0) {
-    uint32_t bound = 0;                                  // fewer threads than k have data: every element
-    if (sh.n >= k) {
-      uint32_t key[kPer], lo = 0xffffffffu, hi = 0;
+  if (n < k) return 0;
+  uint32_t key[kPer], lo = 0xffffffffu, hi = 0;
 #pragma unroll
-      for (int q = 0; q < kPer; ++q) {
-        key[q] = ts.key[lane + 32 * q];
-        if (lane + 32 * q < sh.n) lo = min(lo, key[q]);
-        hi = max(hi, key[q]);
-      }
-      lo = __reduce_min_sync(0xffffffffu, lo);           // count(key >= lo) >= k throughout
-      hi = __reduce_max_sync(0xffffffffu, hi);           // nothing to find above
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2 + 1;
-        uint32_t at = 0;
-#pragma unroll
-        for (int q = 0; q < kPer; ++q) at += key[q] >= mid;
-        at = __reduce_add_sync(0xffffffffu, at);
-        if (at >= k) lo = mid;
-        else hi = mid - 1;
-        if (at >= k && at <= k + k / 4) break;
-      }
-      bound = lo;
-    }
-    if (lane == 0) ts.bound = bound;
+  for (int q = 0; q < kPer; ++q) {
+    key[q] = ts.key[threadIdx.x + 32 * q];
+    if (threadIdx.x + 32 * q < n) lo = min(lo, key[q]);
+    hi = max(hi, key[q]);
   }
+  lo = __reduce_min_sync(0xffffffffu, lo);             // count(key >= lo) >= k throughout
+  hi = __reduce_max_sync(0xffffffffu, hi);             // nothing to find above
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    uint32_t at = 0;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) at += key[q] >= mid;
+    at = __reduce_add_sync(0xffffffffu, at);
+    if (at >= k) lo = mid;
+    else hi = mid - 1;
+    if (at >= k && at <= k + k / 2 + 2) break;
+  }
+  return lo;
+}
+// The block's elements that reach the bound, best first, into out[0 .. k): at most k, then zeros. Only the vectors of
+// threads whose maximum reaches the bound are looked at again, by all warps; what they hold is ranked by counting.
+// ts.hots and ts.count are zero ahead of the barrier that the caller passed last.
+template <class T>
+__device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, uint32_t key, uint32_t bound, uint32_t k,
+                                          TopShared& ts, Key* out) {
+  const uint32_t lane = threadIdx.x & 31;
+  if (threadIdx.x < sh.n && key >= bound) ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
   __syncthreads();
-  const uint32_t bound = ts.bound;
-  if (threadIdx.x < sh.n && ts.key[threadIdx.x] >= bound) ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
-  __syncthreads();
-  const uint32_t hots = ts.hots;
-  for (uint32_t h = warp; h < hots; h += kWarps)
-    for (uint32_t i = ts.hot[h] + lane * kThreads; i < sh.n; i += 32 * kThreads)
-      each_from(sh, sm, i, bound, [&](Key e) {
-        const uint32_t p = atomicAdd(&ts.count, 1u);
-        if (p < kCand) ts.cand[p] = e;
-      });
+  const float thr = bound == 0 ? -INFINITY : key_value(static_cast<Key>(bound) << 32);
+  {
+    // a thread's vectors by as many lanes as it has vectors (a power of two, 32 at most)
+    const uint32_t hots = ts.hots, per_thread = (sh.n + kThreads - 1) / kThreads;
+    const uint32_t wide = per_thread > 16 ? 5u : per_thread > 8 ? 4u : per_thread > 4 ? 3u : per_thread > 2 ? 2u : per_thread > 1 ? 1u : 0u;
+    for (uint32_t h = threadIdx.x >> wide; h < hots; h += kThreads >> wide)
+      for (uint32_t i = ts.hot[h] + (lane & ((1u << wide) - 1)) * kThreads; i < sh.n; i += kThreads << wide)
+        each_from(sh, sm, i, bound, thr, [&](Key e) {
+          const uint32_t p = atomicAdd(&ts.count, 1u);
+          if (p < kCand) ts.cand[p] = e;
+        });
+  }
   __syncthreads();
   uint32_t found = ts.count;
   if (found > kCand) {
@@ -385,9 +412,10 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
     Key lo = static_cast<Key>(bound) << 32, hi = ~0ull;
     while (lo < hi) {
       const Key mid = lo + (hi - lo) / 2 + 1;
+      const uint32_t least = static_cast<uint32_t>(mid >> 32);
       uint32_t mine = 0;
       for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-        each_from(sh, sm, i, static_cast<uint32_t>(mid >> 32), [&](Key e) { mine += e >= mid; });
+        each_from(sh, sm, i, least, key_value(mid), [&](Key e) { mine += e >= mid; });
       mine = __reduce_add_sync(0xffffffffu, mine);
       __syncthreads();
       if (threadIdx.x == 0) ts.count = 0;
@@ -403,7 +431,7 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
     if (threadIdx.x == 0) ts.count = 0;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-      each_from(sh, sm, i, static_cast<uint32_t>(lo >> 32), [&](Key e) {
+      each_from(sh, sm, i, static_cast<uint32_t>(lo >> 32), key_value(lo), [&](Key e) {
         if (e >= lo) ts.cand[atomicAdd(&ts.count, 1u)] = e;
       });
     __syncthreads();
@@ -413,9 +441,14 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
     const Key e = ts.cand[i];
     uint32_t ahead = 0;
 #pragma unroll 4
-    for (uint32_t j = 0; j < found; ++j) ahead += ts.cand[j] > e;
+    for (uint32_t j = 0; j + 1 < found; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(ts.cand + j);
+      ahead += (o.x > e) + (o.y > e);
+    }
+    if (found & 1) ahead += ts.cand[found - 1] > e;
     if (ahead < k) out[ahead] = e;
   }
+  for (uint32_t i = found + threadIdx.x; i < k; i += kThreads) out[i] = 0;
 }
 // Entries of a descending list that are above e.
 __device__ __forceinline__ uint32_t count_above(const Key* list, uint32_t n, Key e) {
@@ -429,7 +462,8 @@ __device__ __forceinline__ uint32_t count_above(const Key* list, uint32_t n, Key
 }
 
 // Block 0 of a row's cluster writes the results: the others send it their statistics and their own
-// best top_k (behind the row in its shared memory) and leave.
+// best top_k (behind the row in its shared memory) and leave. The bound of the selection is the
+// row's: each block proposes one that its part of top_k elements reach, the least of them holds.
 template <class T, bool ENT>
 __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token_scores d, uint32_t share, uint32_t blocks) {
   extern __shared__ uint4 sm[];
@@ -439,15 +473,12 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   const uint32_t rank = blockIdx.x % blocks;           // blocks of a row follow each other, as a cluster's do
   const size_t r = blockIdx.x / blocks;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  const bool first_warp = threadIdx.x < 32;
   Key* lists = reinterpret_cast<Key*>(sm + share);     // [blocks][K]
-  const Share<T> sh(d.logits, r, d.row_stride, V, share, rank);
+  const Share<T> sh(d.logits, r, d.row_stride, V, blocks, rank);
   sh.load(sm);
-  if (K) {
-    if (rank == 0)
-      for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) lists[i] = 0;
-    if (threadIdx.x == 0) ts.hots = ts.count = 0;
-  }
-  if (blocks > 1) cl.barrier_arrive();                 // its wait is where other blocks' memory is first written
+  if (blocks > 1) cluster_arrive(false);               // waited for ahead of the first write to another block
+  if (threadIdx.x == 0) ts.hots = ts.count = 0;
   // the given token's logit comes from memory: it may lie in any block's share
   int32_t lab = -1;
   float xl = 0.0f;
@@ -458,29 +489,47 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   const float c = kLog2e / d.temperature;
   sh.wait();                                           // every thread reads only what it copied itself
   const float tmax = thread_max<T>(sm, sh.n);
-  const Stats ws = warp_stats<T, ENT>(sm, sh.n, tmax, c);
-  if ((threadIdx.x & 31) == 0) ss.warp[threadIdx.x >> 5] = ws;
-  if (K) ts.key[threadIdx.x] = threadIdx.x < sh.n ? order_key(tmax) : 0u;
+  const float wmax = warp_max_nan(tmax);
+  if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
+  const uint32_t key = threadIdx.x < sh.n ? order_key(tmax) : 0u;
+  ts.key[threadIdx.x] = key;
   __syncthreads();
-  if (blocks > 1) cl.barrier_wait();
-  if (threadIdx.x < 32) send_block_stats(ss, c, cl, rank, 1);
-  if (K) block_top(sh, sm, K, ts, (rank == 0 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
+  if (blocks > 1) cluster_wait();
+  if (K) {
+    if (first_warp) {
+      const uint32_t bound = top_bound(ts, sh.n, (K + blocks - 1) / blocks);
+      if (threadIdx.x < blocks) (blocks == 1 ? &ts : cl.map_shared_rank(&ts, threadIdx.x))->bound[rank] = bound;
+    }
+    if (blocks > 1) cluster_arrive(first_warp);        // the sums hide its latency
+  }
+  const float m = block_max(ss);
+  float s, t;
+  warp_sums<T, ENT>(sm, sh.n, m, c, s, t);
+  if ((threadIdx.x & 31) == 0) { ss.s[threadIdx.x >> 5] = s; ss.t[threadIdx.x >> 5] = t; }
+  __syncthreads();
+  if (K && blocks > 1) cluster_wait();
+  if (first_warp) send_block_stats(ss, m, cl, rank, blocks, 1);
+  if (K) {
+    uint32_t bound = ts.bound[0];
+    for (uint32_t b = 1; b < blocks; ++b) bound = min(bound, ts.bound[b]);
+    block_top(sh, sm, key, bound, K, ts, (blocks == 1 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
+  }
   if (blocks > 1) {
-    cl.barrier_arrive();
+    cluster_arrive(first_warp || K != 0);
     if (rank != 0) return;
-    cl.barrier_wait();
+    cluster_wait();
   } else {
     __syncthreads();
   }
-  if (threadIdx.x >= blocks * K && threadIdx.x >= 32) return;
+  if (threadIdx.x >= blocks * K && !first_warp) return;
   const Stats row = row_stats(ss, c, blocks);
-  const double S = row.s, logS = log(S), inv_t = 1.0 / static_cast<double>(d.temperature);
+  const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
   auto logprob = [&](float x) {
-    return S == 0.0 ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - logS);
+    return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
   };
   if (threadIdx.x == 0) {
     if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
-    if (d.entropy) d.entropy[r] = S == 0.0 ? 0.0f : static_cast<float>(logS - row.t * kLn2 / S);
+    if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
     if (d.stats) {
       d.stats[2 * r] = row.m;
       d.stats[2 * r + 1] = row.s;
@@ -488,7 +537,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   }
   for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
     const Key e = lists[i];
-    if (e == 0) continue;                              // a share of fewer than K elements
+    if (e == 0) continue;                              // fewer than K of the block's elements reach the bound
     const uint32_t own = i / K;
     uint32_t ahead = i - own * K;
     for (uint32_t b = 0; b < blocks; ++b)
@@ -516,7 +565,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
   const size_t r = blockIdx.x / parts;
   const uint32_t part = blockIdx.x % parts;
   const uint32_t V = static_cast<uint32_t>(d.vocab);
-  const Share<T> sh(d.logits, r, d.row_stride, V, kThreads * kGradVecs, part);
+  const Share<T> sh(d.logits, r, d.row_stride, V, parts, part);
   T* g = static_cast<T*>(d.dlogits) + r * d.grad_stride;
   uint4 v[kGradVecs];
 #pragma unroll
@@ -589,14 +638,14 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
 }
 
 // ---- distillation ------------------------------------------------------------------------------
-// The teacher's side of one row: thread i < top_k holds entry i, warps without entries skip it. All
-// of it is worked out while the row is on its way to shared memory, in 64 bits: a loss near 0 is a
+// The teacher's side of one row: thread i < top_k holds entry i, warps without entries skip it. It
+// is worked out while the row is on its way to shared memory, in 64 bits: a loss near 0 is a
 // difference of much larger terms.
 struct Entry {
   int32_t id;          // -1: absent (or beyond the list)
   bool first;          // no earlier entry names the token
   float v, x;          // the teacher's value, the student's logit
-  double q, e;         // probability of this entry alone; exp((x - max x) / T) over the entries
+  double q, e;         // exp of the value (over all entries' sum it is q, without a tail); of (x - base) / T
 };
 constexpr int kEntryWarps = kTopMax / 32;
 struct TeacherShared {
@@ -604,55 +653,11 @@ struct TeacherShared {
   double q[kTopMax];
   double z[kEntryWarps], s[kEntryWarps], l[kEntryWarps];
   float v[kEntryWarps], x[kEntryWarps];
-  float A, mt;         // of the gradient, once the row is known
-  double named;        // factor of Entry::e in a named token's gradient
+  float A, mt, named;  // of the gradient, once the row is known; named: factor of Entry::e
+  double inv_z;        // Entry::q to probability
   int bad, dup, empty; // empty: the student's row has no unmasked token
 };
-// Entries and the greatest value; a barrier has to follow.
-__device__ __forceinline__ void teacher_load(const int32_t* ids, const void* vals, uint32_t vdtype, size_t r, uint32_t K,
-                                             TeacherShared& sh, Entry& e) {
-  const uint32_t i = threadIdx.x;
-  e.id = -1;
-  e.v = -INFINITY;
-  e.first = false;
-  if (i >= kTopMax) return;
-  if (i == 0) sh.bad = sh.dup = 0;
-  if (i < K) {
-    e.id = ids[r * K + i];
-    if (e.id >= 0) e.v = load_as_f32(vals, vdtype, r * K + i);
-  }
-  sh.id[i] = e.id;
-  const float top = warp_max_nan(e.v);
-  if ((i & 31) == 0) sh.v[i >> 5] = top;
-}
-// The teacher's exponentials, and which entries are first to name their token; a barrier has to follow.
-__device__ __forceinline__ void teacher_exp(uint32_t V, uint32_t K, bool tail, TeacherShared& sh, Entry& e) {
-  const uint32_t i = threadIdx.x;
-  e.q = 0.0;
-  if ((i & ~31u) >= K) return;
-  if (e.id >= 0) {
-    if (static_cast<uint32_t>(e.id) >= V) sh.bad = 1;
-    uint32_t same = 0;                       // entries before this one that name its token
-    const int4* id4 = reinterpret_cast<const int4*>(sh.id);
-    for (uint32_t j = 0; 4 * j < i; ++j) {
-      const int4 o = id4[j];
-      same += (o.x == e.id && 4 * j < i) + (o.y == e.id && 4 * j + 1 < i) + (o.z == e.id && 4 * j + 2 < i) +
-              (o.w == e.id && 4 * j + 3 < i);
-    }
-    e.first = same == 0;
-    if (same) sh.dup = 1;
-    double shift = 0.0;
-    if (!tail) {
-      float vm = sh.v[0];
-      for (uint32_t w = 1; w < kEntryWarps; ++w) vm = max_nan(vm, sh.v[w]);
-      shift = vm == -INFINITY ? 0.0 : vm;
-    }
-    e.q = exp(e.v - shift);
-  }
-  const double z = warp_sum(e.q);
-  const float x = warp_max_nan(e.x);
-  if ((i & 31) == 0) { sh.z[i >> 5] = z; sh.x[i >> 5] = x; }
-}
+__device__ __forceinline__ bool entry_warp(uint32_t K) { return (threadIdx.x & ~31u) < K; }
 __device__ __forceinline__ double entry_sum(const double* part, uint32_t K) {
   double s = part[0];
   for (uint32_t w = 1; 32 * w < K; ++w) s += part[w];
@@ -663,11 +668,44 @@ __device__ __forceinline__ float entry_max(const float* part, uint32_t K) {
   for (uint32_t w = 1; 32 * w < K; ++w) m = max_nan(m, part[w]);
   return m;
 }
+// Behind the barrier that made the entries visible, ahead of another: the teacher's exponentials, which entries are
+// first to name their token, and the student's exponentials of those against `base`.
+__device__ __forceinline__ void entries_exp(uint32_t V, uint32_t K, bool tail, double inv_t, float base, TeacherShared& sh,
+                                            Entry& e) {
+  const uint32_t i = threadIdx.x;
+  if (e.id >= 0) {
+    if (static_cast<uint32_t>(e.id) >= V) sh.bad = 1;
+    uint32_t same = 0;                       // entries before this one that name its token
+    const int4* id4 = reinterpret_cast<const int4*>(sh.id);
+#pragma unroll 4
+    for (uint32_t j = 0; 4 * j < i; ++j) {
+      const int4 o = id4[j];
+      same += (o.x == e.id && 4 * j < i) + (o.y == e.id && 4 * j + 1 < i) + (o.z == e.id && 4 * j + 2 < i) +
+              (o.w == e.id && 4 * j + 3 < i);
+    }
+    e.first = same == 0;
+    if (same) sh.dup = 1;
+    float shift = tail ? 0.0f : entry_max(sh.v, K);
+    if (shift == -INFINITY) shift = 0.0f;
+    e.q = exp(static_cast<double>(e.v) - shift);
+    if (e.first && e.x != -INFINITY) e.e = exp((static_cast<double>(e.x) - base) * inv_t);
+  }
+  sh.q[i] = e.q;
+  const double z = warp_sum(e.q), s = warp_sum(e.e);
+  if ((i & 31) == 0) { sh.z[i >> 5] = z; sh.s[i >> 5] = s; }
+}
 // Sum of the entries' probabilities and the teacher's mass on all other tokens.
-__device__ __forceinline__ void teacher_mass(const TeacherShared& sh, uint32_t K, bool tail, double& qsum, double& rest) {
-  const double z = entry_sum(sh.z, K);
+__device__ __forceinline__ void teacher_mass(double z, bool tail, double& qsum, double& rest) {
   qsum = tail ? z : z == 0.0 ? 0.0 : z != z ? z : 1.0;
   rest = tail && qsum < 1.0 ? 1.0 - qsum : 0.0;
+}
+// exp(d / T) for d <= 0 with the rounding of the exponent made good
+__device__ __forceinline__ float exp_of(float d, double log2e_t) {
+  const double y = d * log2e_t;
+  const float hi = static_cast<float>(y);
+  const float lo = static_cast<float>(y - hi);
+  const float e = ex2(hi);
+  return e == 0.0f ? 0.0f : fmaf(e, lo * static_cast<float>(kLn2), e);
 }
 
 enum Mode { kLoss, kStep, kBackward };
@@ -675,21 +713,28 @@ struct DistillArgs {
   seeml_b200_distill_topk d;
   const float* saved_in;       // kBackward
   const float* upstream;       // kBackward: d loss / d row_loss
+  double inv_t, log2e_t;       // 1 / T, log2(e) / T
 };
 
 // Gradient of a row: unnamed tokens get A exp((x - mt) / T) with one factor A for the row, named ones
-// up / T (p Q - q). S is the sum over all tokens at maximum m, st that over the unnamed at mt.
-__device__ __forceinline__ void distill_factors(TeacherShared& th, float up_t, double qsum, double rest, float mt, float st,
-                                                float m, float S, float entry_m, float inv_t) {
+// up / T (p Q - q). S is the sum over all tokens at maximum m, st that over the unnamed at mt; the entries'
+// exponentials were taken against `base`.
+__device__ __forceinline__ void distill_factors(TeacherShared& th, uint32_t K, bool tail, float up_t, float mt, float st,
+                                                float m, float S, float base, double log2e_t) {
+  double qsum, rest;
+  const double z = entry_sum(th.z, K);
+  teacher_mass(z, tail, qsum, rest);
   if (st == 0.0f) rest = 0.0;
   const float Q = static_cast<float>(qsum + rest);
+  const float inv_s = 1.0f / S;
   float A = 0.0f;
-  if (st != 0.0f && S != 0.0f) A = up_t * (Q * expf((mt - m) * inv_t) / S - static_cast<float>(rest) / st);
+  if (st != 0.0f && S != 0.0f) A = up_t * (Q * exp_of(mt - m, log2e_t) * inv_s - static_cast<float>(rest) / st);
   if (th.bad || S != S) A = nan_f();
   th.A = A;
-  th.empty = S == 0.0f;
   th.mt = mt == -INFINITY ? 0.0f : mt;
-  th.named = S != S ? S : S == 0.0f || entry_m == -INFINITY ? 0.0 : static_cast<double>(Q * expf((entry_m - m) * inv_t) / S);
+  th.named = S != S ? S : S == 0.0f || base == -INFINITY ? 0.0f : Q * exp_of(base - m, log2e_t) * inv_s;
+  th.empty = S == 0.0f;
+  th.inv_z = tail ? 1.0 : z == 0.0 ? 0.0 : 1.0 / z;
 }
 
 template <class T, int MODE>
@@ -703,11 +748,18 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
   const uint32_t rank = blockIdx.x % blocks;           // blocks of a row follow each other, as a cluster's do
   const size_t r = blockIdx.x / blocks;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
-  const bool tail = d.tail != 0;
-  const Share<T> sh(d.logits, r, d.row_stride, V, share, rank);
+  const bool tail = d.tail != 0, first_warp = threadIdx.x < 32;
+  const Share<T> sh(d.logits, r, d.row_stride, V, blocks, rank);
   T* g = MODE != kLoss ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
   const bool same = MODE != kLoss && (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
+  // the row's weight and its entries arrive together; the row is only asked for if it counts
   const float w = MODE == kBackward ? a.upstream[r] : d.row_weight ? d.row_weight[r] : 1.0f;
+  Entry e{-1, false, -INFINITY, -INFINITY, 0.0, 0.0};
+  if (threadIdx.x < K) {
+    e.id = d.teacher_id[r * K + threadIdx.x];
+    const float v = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * K + threadIdx.x);
+    if (e.id >= 0) e.v = v;
+  }
   if (w == 0.0f) {                                     // the whole cluster leaves here
     if (MODE != kLoss) {
       float2 f[E / 2];
@@ -729,90 +781,67 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
     return;
   }
   sh.load(sm);
-  if (MODE != kBackward && blocks > 1) cl.barrier_arrive();    // waited for ahead of the first write to another block
-  Entry e;
-  teacher_load(d.teacher_id, d.teacher_logprob, d.teacher_dtype, r, K, th, e);
-  e.x = -INFINITY;
-  // read here, ahead of the cluster's barrier: in place, another block may overwrite it behind that
+  if (MODE != kBackward && blocks > 1) cluster_arrive(false);  // waited for ahead of the first write to another block
+  const bool entries = entry_warp(K);
+  // Read here, ahead of the cluster's barrier: in place, another block may overwrite it behind that. The backward
+  // call has no such barrier and needs only the entries of its own share, which it finds in shared memory.
   if (MODE != kBackward && e.id >= 0 && static_cast<uint32_t>(e.id) < V) e.x = Ty<T>::to(sh.x[e.id]);
+  if (threadIdx.x == 0) th.bad = th.dup = 0;
+  if (entries) {
+    th.id[threadIdx.x] = e.id;
+    const float vm = warp_max_nan(e.v), xm = warp_max_nan(e.x);
+    if ((threadIdx.x & 31) == 0) { th.v[threadIdx.x >> 5] = vm; th.x[threadIdx.x >> 5] = xm; }
+  }
   __syncthreads();
-  teacher_exp(V, K, tail, th, e);
-  const float c = kLog2e / d.temperature, inv_t = 1.0f / d.temperature;
+  const float base = MODE == kBackward ? 0.0f : entry_max(th.x, K);
+  if (entries) entries_exp(V, K, tail, a.inv_t, base, th, e);
+  const float c = kLog2e / d.temperature;
   sh.wait();
   __syncthreads();
   // named tokens leave the parked row: what is left is the student's tail, summed without a difference
   const bool bad = th.bad != 0;
   const int at = e.id >= 0 && !bad ? sh.local(e.id) : -1;
-  e.e = 0.0;
-  float entry_m = -INFINITY;
-  if ((threadIdx.x & ~31u) < K) {
-    if (MODE == kBackward) {
-      entry_m = 0.0f;                                  // Entry::e is taken against the row's maximum below
-      if (at >= 0) e.x = Ty<T>::to(reinterpret_cast<T*>(sm)[at]);
-      __syncwarp();
-    } else {
-      entry_m = entry_max(th.x, K);
-    }
-    if (!tail) {
-      const double z = entry_sum(th.z, K);
-      e.q = z == 0.0 ? 0.0 : e.q / z;
-    }
-    th.q[threadIdx.x] = e.q;
+  if (MODE == kBackward) {
+    if (at >= 0) e.x = Ty<T>::to(reinterpret_cast<T*>(sm)[at]);
+    __syncthreads();                                   // two entries may name one token: both have read it
   }
-  if (MODE == kBackward) __syncthreads();              // two entries may name one token: both have read it
   if (at >= 0) reinterpret_cast<T*>(sm)[at] = Ty<T>::from(-INFINITY);
-  if (MODE != kBackward && (threadIdx.x & ~31u) < K) {
-    const double t64 = 1.0 / static_cast<double>(d.temperature);
-    const double y = (static_cast<double>(e.x) - entry_m) * t64;
-    if (e.first && !bad && e.x != -INFINITY) e.e = exp(y);
-    double l = 0.0;                                    // sum of q (ln q - (x - max) / T)
-    if (e.q != 0.0) {
-      const double log_q = tail ? e.v : e.v - static_cast<double>(entry_max(th.v, K)) - log(entry_sum(th.z, K));
-      l = e.x == -INFINITY ? INFINITY : e.q * (log_q - y);
-    }
-    const double s = warp_sum(e.e);
-    l = warp_sum(l);
-    if ((threadIdx.x & 31) == 0) { th.s[threadIdx.x >> 5] = s; th.l[threadIdx.x >> 5] = l; }
-  }
   __syncthreads();
-  double qsum, rest;
-  const float up_t = (MODE == kBackward ? 1.0f : d.scale) * w * inv_t;
+  const float up_t = (MODE == kBackward ? 1.0f : d.scale) * w / d.temperature;
   if (MODE != kBackward) {
-    const float tmax = thread_max<T>(sm, sh.n);
-    const Stats ws = warp_stats<T, false>(sm, sh.n, tmax, c);
-    if ((threadIdx.x & 31) == 0) ss.warp[threadIdx.x >> 5] = ws;
+    const float wmax = warp_max_nan(thread_max<T>(sm, sh.n));
+    if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
     __syncthreads();
-    if (blocks > 1) cl.barrier_wait();
-    if (threadIdx.x < 32) send_block_stats(ss, c, cl, rank, MODE == kLoss ? 1 : blocks);
+    const float bm = block_max(ss);
+    float s, t;
+    warp_sums<T, false>(sm, sh.n, bm, c, s, t);
+    if ((threadIdx.x & 31) == 0) { ss.s[threadIdx.x >> 5] = s; ss.t[threadIdx.x >> 5] = t; }
+    __syncthreads();
+    if (blocks > 1) cluster_wait();
+    if (first_warp) send_block_stats(ss, bm, cl, rank, blocks, MODE == kLoss ? 1 : blocks);
     if (blocks > 1) {
-      cl.barrier_arrive();
+      cluster_arrive(first_warp);
       if (MODE == kLoss && rank != 0) return;
-      cl.barrier_wait();
+      cluster_wait();
     } else {
       __syncthreads();
     }
     if (MODE == kStep) {
       if (threadIdx.x == 0) {
         const Stats row = row_stats(ss, c, blocks);
-        const float m = max_nan(row.m, entry_m);
+        const float m = max_nan(row.m, base), es = static_cast<float>(entry_sum(th.s, K));
         float S = 0.0f;
-        if (row.s != 0.0f) S = row.s * expf((row.m - m) * inv_t);
-        const float es = static_cast<float>(entry_sum(th.s, K));
-        if (es != 0.0f) S += es * expf((entry_m - m) * inv_t);
+        if (row.s != 0.0f) S = row.s * exp_of(row.m - m, a.log2e_t);
+        if (es != 0.0f) S += es * exp_of(base - m, a.log2e_t);
         if (m != m) S = nan_f();
-        teacher_mass(th, K, tail, qsum, rest);
-        distill_factors(th, up_t, qsum, rest, row.m, row.s, m, S, entry_m, inv_t);
+        distill_factors(th, K, tail, up_t, row.m, row.s, m, S, base, a.log2e_t);
       }
       __syncthreads();
     }
   } else {
     const float* sv = a.saved_in + 4 * r;
-    const float m = sv[2];
-    if (at >= 0 && e.x != -INFINITY) e.e = exp((static_cast<double>(e.x) - m) / d.temperature);
-    if (threadIdx.x == 0) {
-      teacher_mass(th, K, tail, qsum, rest);
-      distill_factors(th, up_t, qsum, rest, sv[0], sv[1], m, sv[3], m, inv_t);
-    }
+    if (threadIdx.x == 0) distill_factors(th, K, tail, up_t, sv[0], sv[1], sv[2], sv[3], sv[2], a.log2e_t);
+    if (at >= 0 && e.x != -INFINITY) e.e = exp((static_cast<double>(e.x) - sv[2]) * a.inv_t);
     __syncthreads();
   }
   if (MODE != kLoss) {
@@ -854,27 +883,42 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
         for (uint32_t j = 0; j < K; ++j)
           if (th.id[j] == e.id) q += th.q[j];
       }
-      g[e.id] = Ty<T>::from(th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named - q)));
+      g[e.id] = Ty<T>::from(th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named - q * th.inv_z)));
     }
   }
-  if (MODE != kBackward && rank == 0 && threadIdx.x == 0) {
-    const Stats row = row_stats(ss, c, blocks);
-    const double t64 = 1.0 / static_cast<double>(d.temperature), st = row.s, es = entry_sum(th.s, K);
-    const float m = max_nan(row.m, entry_m);
-    double S = 0.0;
-    if (st != 0.0) S = st * exp((static_cast<double>(row.m) - m) * t64);
-    if (es != 0.0) S += es * exp((static_cast<double>(entry_m) - m) * t64);
-    if (m != m) S = nan_f();
-    teacher_mass(th, K, tail, qsum, rest);
-    const double logS = log(S);
-    double l = entry_sum(th.l, K);
-    if (qsum != 0.0) l += qsum * ((static_cast<double>(m) - entry_m) * t64 + logS);
-    if (qsum != 0.0 && S == 0.0) l = INFINITY;
-    if (rest > 0.0 && st != 0.0) l += rest * (log(rest) - ((static_cast<double>(row.m) - m) * t64 + log(st) - logS));
-    d.row_loss[r] = bad ? nan_f() : static_cast<float>(l);
-    if (d.saved) {
-      float* sv = d.saved + 4 * r;
-      sv[0] = row.m; sv[1] = row.s; sv[2] = m; sv[3] = static_cast<float>(S);
+  // the loss, behind the gradient that nobody waits for: sum of q (ln q - (x - base) / T) over the entries first
+  if (MODE != kBackward && rank == 0) {
+    const double z = entry_sum(th.z, K), log_z = ln_sum(static_cast<float>(z));
+    if (entries) {
+      double l = 0.0;
+      if (e.q != 0.0) {
+        const double log_q = tail ? e.v : static_cast<double>(e.v) - entry_max(th.v, K) - log_z;
+        l = e.x == -INFINITY ? INFINITY : (tail ? e.q : e.q / z) * (log_q - (static_cast<double>(e.x) - base) * a.inv_t);
+      }
+      l = warp_sum(l);
+      if ((threadIdx.x & 31) == 0) th.l[threadIdx.x >> 5] = l;
+    }
+    if (K > 32) __syncthreads();
+    if (threadIdx.x == 0) {
+      const Stats row = row_stats(ss, c, blocks);
+      const float m = max_nan(row.m, base), st = row.s, es = static_cast<float>(entry_sum(th.s, K));
+      float S = 0.0f;
+      if (st != 0.0f) S = st * exp_of(row.m - m, a.log2e_t);
+      if (es != 0.0f) S += es * exp_of(base - m, a.log2e_t);
+      if (m != m) S = nan_f();
+      double qsum, rest;
+      teacher_mass(z, tail, qsum, rest);
+      const double log_s = ln_sum(S);
+      double l = entry_sum(th.l, K);
+      if (qsum != 0.0) l += qsum * ((static_cast<double>(m) - base) * a.inv_t + log_s);
+      if (qsum != 0.0 && S == 0.0f) l = INFINITY;
+      if (rest > 0.0 && st != 0.0f)
+        l += rest * (log(rest) - ((static_cast<double>(row.m) - m) * a.inv_t + ln_sum(st) - log_s));
+      d.row_loss[r] = bad ? nan_f() : static_cast<float>(l);
+      if (d.saved) {
+        float* sv = d.saved + 4 * r;
+        sv[0] = row.m; sv[1] = st; sv[2] = m; sv[3] = S;
+      }
     }
   }
 }
@@ -972,9 +1016,13 @@ int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st) {
     return 1;
   });
 }
+static DistillArgs distill_args(const seeml_b200_distill_topk& d) {
+  const double inv_t = 1.0 / static_cast<double>(d.temperature);
+  return DistillArgs{d, nullptr, nullptr, inv_t, inv_t / kLn2};
+}
 int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
   const Split s = split_row(d.rows, d.vocab, elem_bytes(d.dtype));
-  const DistillArgs a{d, nullptr, nullptr};
+  const DistillArgs a = distill_args(d);
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
     return d.dlogits ? launch_rows<distill_kernel<T, kStep>>(d.rows, s, true, 0, st, a)
@@ -983,20 +1031,21 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
 }
 int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
   const Split s = split_row(b.rows, b.vocab, elem_bytes(b.dtype));
-  DistillArgs a{};
-  a.d.logits = b.logits;
-  a.d.teacher_id = b.teacher_id;
-  a.d.teacher_logprob = b.teacher_logprob;
-  a.d.dlogits = b.dlogits;
-  a.d.rows = b.rows;
-  a.d.vocab = b.vocab;
-  a.d.row_stride = b.row_stride;
-  a.d.grad_stride = b.grad_stride;
-  a.d.dtype = b.dtype;
-  a.d.teacher_dtype = b.teacher_dtype;
-  a.d.top_k = b.top_k;
-  a.d.tail = b.tail;
-  a.d.temperature = b.temperature;
+  seeml_b200_distill_topk d{};
+  d.logits = b.logits;
+  d.teacher_id = b.teacher_id;
+  d.teacher_logprob = b.teacher_logprob;
+  d.dlogits = b.dlogits;
+  d.rows = b.rows;
+  d.vocab = b.vocab;
+  d.row_stride = b.row_stride;
+  d.grad_stride = b.grad_stride;
+  d.dtype = b.dtype;
+  d.teacher_dtype = b.teacher_dtype;
+  d.top_k = b.top_k;
+  d.tail = b.tail;
+  d.temperature = b.temperature;
+  DistillArgs a = distill_args(d);
   a.saved_in = b.saved;
   a.upstream = b.drow_loss;
   return by_type(b.dtype, [&](auto t) {
