@@ -66,8 +66,24 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 
 // ---- a 16-byte vector of each logits type ------------------------------------------------------
 template <class T> struct Ty;
+template <class T>
+__device__ __forceinline__ void set_half(uint32_t (&w)[4], int q, T x) {
+  const uint32_t b = *reinterpret_cast<const uint16_t*>(&x);
+  w[q / 2] = q & 1 ? (w[q / 2] & 0x0000ffffu) | (b << 16) : (w[q / 2] & 0xffff0000u) | b;
+}
+__device__ __forceinline__ void mask_halves(uint4& v, uint32_t bits, uint32_t masked) {
+  auto one = [&](uint32_t w, uint32_t two) {
+    const uint32_t keep = (two & 1u ? 0u : 0x0000ffffu) | (two & 2u ? 0u : 0xffff0000u);
+    return (w & keep) | (masked & ~keep);
+  };
+  v.x = one(v.x, bits);
+  v.y = one(v.y, bits >> 2);
+  v.z = one(v.z, bits >> 4);
+  v.w = one(v.w, bits >> 6);
+}
 template <> struct Ty<float> {
   static constexpr int E = 4;
+  static constexpr uint32_t kMasked = 0xff800000u;     // -inf in every element of a word
   static __device__ __forceinline__ float to(float x) { return x; }
   static __device__ __forceinline__ float from(float x) { return x; }
   static __device__ __forceinline__ void unpack(const uint4& v, float2 (&f)[2]) {
@@ -77,12 +93,20 @@ template <> struct Ty<float> {
   static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
     return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
   }
+  static __device__ __forceinline__ void set(uint32_t (&w)[4], int q, float x) { w[q] = __float_as_uint(x); }
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) {
+    if (bits & 1u) v.x = kMasked;
+    if (bits & 2u) v.y = kMasked;
+    if (bits & 4u) v.z = kMasked;
+    if (bits & 8u) v.w = kMasked;
+  }
   static __device__ __forceinline__ float vmax(const uint4& v) {
     return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
 };
 template <> struct Ty<__nv_bfloat16> {
   static constexpr int E = 8;
+  static constexpr uint32_t kMasked = 0xff80ff80u;
   static __device__ __forceinline__ float to(__nv_bfloat16 x) { return __bfloat162float(x); }
   static __device__ __forceinline__ __nv_bfloat16 from(float x) { return __float2bfloat16(x); }
   static __device__ __forceinline__ float2 two(uint32_t w) {
@@ -98,6 +122,8 @@ template <> struct Ty<__nv_bfloat16> {
   static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
     return make_uint4(bits(f[0]), bits(f[1]), bits(f[2]), bits(f[3]));
   }
+  static __device__ __forceinline__ void set(uint32_t (&w)[4], int q, __nv_bfloat16 x) { set_half(w, q, x); }
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) { mask_halves(v, bits, kMasked); }
   static __device__ __forceinline__ float vmax(const uint4& v) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
     const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
@@ -106,6 +132,7 @@ template <> struct Ty<__nv_bfloat16> {
 };
 template <> struct Ty<__half> {
   static constexpr int E = 8;
+  static constexpr uint32_t kMasked = 0xfc00fc00u;
   static __device__ __forceinline__ float to(__half x) { return __half2float(x); }
   static __device__ __forceinline__ __half from(float x) { return __float2half(x); }
   static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
@@ -119,6 +146,8 @@ template <> struct Ty<__half> {
   static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
     return make_uint4(bits(f[0]), bits(f[1]), bits(f[2]), bits(f[3]));
   }
+  static __device__ __forceinline__ void set(uint32_t (&w)[4], int q, __half x) { set_half(w, q, x); }
+  static __device__ __forceinline__ void mask(uint4& v, uint32_t bits) { mask_halves(v, bits, kMasked); }
   static __device__ __forceinline__ float vmax(const uint4& v) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
     const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
@@ -317,6 +346,115 @@ __device__ __forceinline__ double ln_sum(float S) {
   return e * kLn2 + static_cast<double>(logf(f));
 }
 
+// ---- a row streamed by one block -------------------------------------------------------------------
+// A call of many rows gives each row to one block that reads it straight into registers, kBatch
+// vectors per thread at a time with the next batch in flight behind the one being summed; several
+// blocks live on an SM, so that the ends of rows hide behind the middle of others. Nothing couples
+// the blocks: a cluster has to find room for all its blocks at once, which left SMs idle.
+constexpr int kBatch = 4;
+constexpr uint32_t kBatchVecs = kBatch * kThreads;
+// Vector i of the row, -inf beyond the row's ends.
+template <class T>
+__device__ __forceinline__ uint4 row_vec(const Share<T>& sh, uint32_t i) {
+  if (sh.whole(i)) return *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
+  uint4 v = make_uint4(Ty<T>::kMasked, Ty<T>::kMasked, Ty<T>::kMasked, Ty<T>::kMasked);
+  if (i < sh.n) {
+    const int j = sh.elem(i);
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int q = 0; q < Ty<T>::E; ++q)
+      if (j + q >= 0 && j + q < static_cast<int>(sh.V)) Ty<T>::set(w, q, sh.x[j + q]);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+template <class T>
+__device__ __forceinline__ void row_batch(const Share<T>& sh, uint32_t b, uint4 (&v)[kBatch]) {
+  const uint32_t i = b * kBatchVecs + threadIdx.x;
+  if (b * kBatchVecs >= sh.lo && (b + 1) * kBatchVecs <= sh.hi) {
+    const uint4* p = reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = p[u * kThreads];
+  } else {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = row_vec(sh, i + u * kThreads);
+  }
+}
+template <class T, bool ENT, bool CLAMP>
+__device__ __forceinline__ void batch_sums(const uint4 (&v)[kBatch], float shift, float c, float& s_out, float& t_out) {
+  constexpr int H = Ty<T>::E / 2;
+  const float2 sh2 = make_float2(-shift, -shift), c2 = make_float2(c, c);
+  float2 s[2], t[2];
+  s[0] = s[1] = t[0] = t[1] = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) {
+    float2 f[H];
+    Ty<T>::unpack(v[u], f);
+#pragma unroll
+    for (int q = 0; q < H; ++q) {
+      float2 y = mul2(add2(f[q], sh2), c2);
+      if (CLAMP) {
+        y.x = max_nan(y.x, -200.0f);
+        y.y = max_nan(y.y, -200.0f);
+      }
+      const float2 e = make_float2(ex2(y.x), ex2(y.y));
+      s[q & 1] = add2(s[q & 1], e);
+      if (ENT) t[q & 1] = fma2(e, y, t[q & 1]);
+    }
+  }
+  s[0] = add2(s[0], s[1]);
+  s_out = s[0].x + s[0].y;
+  if (ENT) {
+    t[0] = add2(t[0], t[1]);
+    t_out = t[0].x + t[0].y;
+  }
+}
+// Statistics of this thread's vectors of the row, in one pass with a running maximum. named: a byte per vector whose
+// bits are the elements to leave out, the bytes of a thread's batch in one word (NULL: none).
+template <class T, bool ENT>
+__device__ __forceinline__ Stats stream_stats(const Share<T>& sh, float c, const uint32_t* named) {
+  Stats a{-INFINITY, 0.0f, 0.0f};
+  const uint32_t batches = (sh.n + kBatchVecs - 1) / kBatchVecs;
+  uint4 v[kBatch];
+  row_batch(sh, 0, v);
+  for (uint32_t b = 0; b < batches; ++b) {
+    uint4 next[kBatch];
+    if (b + 1 < batches) row_batch(sh, b + 1, next);
+    if (named) {
+      const uint32_t w = named[b * kThreads + threadIdx.x];
+      if (w) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+          if ((w >> (8 * u)) & 0xffu) Ty<T>::mask(v[u], (w >> (8 * u)) & 0xffu);
+      }
+    }
+    float m = Ty<T>::vmax(v[0]);
+#pragma unroll
+    for (int u = 1; u < kBatch; ++u) m = max_nan(m, Ty<T>::vmax(v[u]));
+    m = max_nan(m, a.m);
+    const float shift = m == -INFINITY ? 0.0f : m;
+    float s, t = 0.0f;
+    batch_sums<T, ENT, false>(v, shift, c, s, t);
+    if (ENT && t != t) batch_sums<T, ENT, true>(v, shift, c, s, t);       // a masked token: 0 * -inf
+    const float y = max_nan((a.m - shift) * c, -200.0f), f = ex2(y);      // the sums so far, against the new maximum
+    if (ENT) a.t = (a.t + a.s * y) * f + t;
+    a.s = a.s * f + s;
+    a.m = m;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = next[u];
+  }
+  return a;
+}
+// The block's statistics from its threads', into sh.block[0] behind the caller's next barrier. Contains a barrier, ahead
+// of which sh.m has to be written.
+template <bool ENT>
+__device__ __forceinline__ void join_threads(StatsShared& sh, Stats a, float c, float m) {
+  const float y = max_nan((a.m - (m == -INFINITY ? 0.0f : m)) * c, -200.0f), f = ex2(y);
+  float t = ENT ? warp_sum((a.t + a.s * y) * f) : 0.0f;
+  const float s = warp_sum(a.s * f);
+  if ((threadIdx.x & 31) == 0) { sh.s[threadIdx.x >> 5] = s; sh.t[threadIdx.x >> 5] = t; }
+}
+
 // ---- token scores ------------------------------------------------------------------------------
 // Order of the alternatives as one integer: greater logit first (-0 equals +0, NaN above all),
 // then the lower index. No two elements of a row share a value; 0 is below all.
@@ -341,19 +479,21 @@ struct TopShared {
 };
 // Calls f(key) for the elements of vector i whose key is at least `least` (thr: the value of that key).
 template <class T, class F>
-__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4* sm, uint32_t i, uint32_t least, float thr, F f) {
+__device__ __forceinline__ void each_from(const Share<T>& sh, const uint4& vec, uint32_t i, uint32_t least, float thr, F f) {
   float2 e[Ty<T>::E / 2];
-  Ty<T>::unpack(sm[i], e);
+  Ty<T>::unpack(vec, e);
   uint32_t hit = 0;
 #pragma unroll
   for (int q = 0; q < Ty<T>::E; ++q)
     if (!((q & 1 ? e[q / 2].y : e[q / 2].x) < thr)) hit |= 1u << q;        // NaN passes
   const int j = sh.elem(i);
-  const T* v = reinterpret_cast<const T*>(sm + i);
   while (hit) {
     const int q = __ffs(hit) - 1;
     hit &= hit - 1;
-    const float x = Ty<T>::to(v[q]);
+    float x = e[0].x;
+#pragma unroll
+    for (int p = 1; p < Ty<T>::E; ++p)
+      if (p == q) x = p & 1 ? e[p / 2].y : e[p / 2].x;
     if (order_key(x) >= least && j + q >= 0 && j + q < static_cast<int>(sh.V)) f(rank_key(x, j + q));
   }
 }
@@ -384,11 +524,12 @@ __device__ __forceinline__ uint32_t top_bound(const TopShared& ts, uint32_t n, u
   return lo;
 }
 // The block's elements that reach the bound, best first, into out[0 .. k): at most k, then zeros. Only the vectors of
-// threads whose maximum reaches the bound are looked at again, by all warps; what they hold is ranked by counting.
+// threads whose maximum reaches the bound are looked at again (vec(i) brings vector i), by all warps; what they hold
+// is ranked by counting.
 // ts.hots and ts.count are zero ahead of the barrier that the caller passed last.
-template <class T>
-__device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, uint32_t key, uint32_t bound, uint32_t k,
-                                          TopShared& ts, Key* out) {
+template <class T, class Vec>
+__device__ __forceinline__ void block_top(const Share<T>& sh, Vec vec, uint32_t key, uint32_t bound, uint32_t k, TopShared& ts,
+                                          Key* out) {
   const uint32_t lane = threadIdx.x & 31;
   if (threadIdx.x < sh.n && key >= bound) ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
   __syncthreads();
@@ -399,7 +540,7 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
     const uint32_t wide = per_thread > 16 ? 5u : per_thread > 8 ? 4u : per_thread > 4 ? 3u : per_thread > 2 ? 2u : per_thread > 1 ? 1u : 0u;
     for (uint32_t h = threadIdx.x >> wide; h < hots; h += kThreads >> wide)
       for (uint32_t i = ts.hot[h] + (lane & ((1u << wide) - 1)) * kThreads; i < sh.n; i += kThreads << wide)
-        each_from(sh, sm, i, bound, thr, [&](Key e) {
+        each_from(sh, vec(i), i, bound, thr, [&](Key e) {
           const uint32_t p = atomicAdd(&ts.count, 1u);
           if (p < kCand) ts.cand[p] = e;
         });
@@ -415,7 +556,7 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
       const uint32_t least = static_cast<uint32_t>(mid >> 32);
       uint32_t mine = 0;
       for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-        each_from(sh, sm, i, least, key_value(mid), [&](Key e) { mine += e >= mid; });
+        each_from(sh, vec(i), i, least, key_value(mid), [&](Key e) { mine += e >= mid; });
       mine = __reduce_add_sync(0xffffffffu, mine);
       __syncthreads();
       if (threadIdx.x == 0) ts.count = 0;
@@ -431,7 +572,7 @@ __device__ __forceinline__ void block_top(const Share<T>& sh, const uint4* sm, u
     if (threadIdx.x == 0) ts.count = 0;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-      each_from(sh, sm, i, static_cast<uint32_t>(lo >> 32), key_value(lo), [&](Key e) {
+      each_from(sh, vec(i), i, static_cast<uint32_t>(lo >> 32), key_value(lo), [&](Key e) {
         if (e >= lo) ts.cand[atomicAdd(&ts.count, 1u)] = e;
       });
     __syncthreads();
@@ -459,6 +600,37 @@ __device__ __forceinline__ uint32_t count_above(const Key* list, uint32_t n, Key
     else hi = mid;
   }
   return lo;
+}
+
+// The results of a row from its statistics and its blocks' lists of alternatives.
+__device__ __forceinline__ void write_scores(const seeml_b200_token_scores& d, size_t r, const Stats& row, int32_t lab, float xl,
+                                             const Key* lists, uint32_t blocks) {
+  const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  if (threadIdx.x >= blocks * K && threadIdx.x >= 32) return;
+  const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
+  auto logprob = [&](float x) {
+    return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
+  };
+  if (threadIdx.x == 0) {
+    if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
+    if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
+    if (d.stats) {
+      d.stats[2 * r] = row.m;
+      d.stats[2 * r + 1] = row.s;
+    }
+  }
+  for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
+    const Key e = lists[i];
+    if (e == 0) continue;                              // fewer than K of the block's elements reach the bound
+    const uint32_t own = i / K;
+    uint32_t ahead = i - own * K;
+    for (uint32_t b = 0; b < blocks; ++b)
+      if (b != own) ahead += count_above(lists + b * K, K, e);
+    if (ahead < K) {
+      d.top_id[r * K + ahead] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
+      d.top_logprob[r * K + ahead] = logprob(key_value(e));
+    }
+  }
 }
 
 // Block 0 of a row's cluster writes the results: the others send it their statistics and their own
@@ -512,7 +684,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   if (K) {
     uint32_t bound = ts.bound[0];
     for (uint32_t b = 1; b < blocks; ++b) bound = min(bound, ts.bound[b]);
-    block_top(sh, sm, key, bound, K, ts, (blocks == 1 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
+    block_top(sh, [&](uint32_t i) { return sm[i]; }, key, bound, K, ts, (blocks == 1 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
   }
   if (blocks > 1) {
     cluster_arrive(first_warp || K != 0);
@@ -521,32 +693,45 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   } else {
     __syncthreads();
   }
-  if (threadIdx.x >= blocks * K && !first_warp) return;
-  const Stats row = row_stats(ss, c, blocks);
-  const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
-  auto logprob = [&](float x) {
-    return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
-  };
-  if (threadIdx.x == 0) {
-    if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
-    if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
-    if (d.stats) {
-      d.stats[2 * r] = row.m;
-      d.stats[2 * r + 1] = row.s;
-    }
+  write_scores(d, r, row_stats(ss, c, blocks), lab, xl, lists, blocks);
+}
+
+// The same of a row that one block streams; the selection reads the few vectors it needs a second time (from L2).
+template <class T, bool ENT>
+__global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_b200_token_scores d) {
+  __shared__ StatsShared ss;
+  __shared__ TopShared ts;
+  __shared__ Key list[kTopMax];
+  cg::cluster_group cl = cg::this_cluster();
+  const size_t r = blockIdx.x;
+  const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  const bool first_warp = threadIdx.x < 32;
+  const Share<T> sh(d.logits, r, d.row_stride, V, 1, 0);
+  if (threadIdx.x == 0) ts.hots = ts.count = 0;
+  int32_t lab = -1;
+  float xl = 0.0f;
+  if (threadIdx.x == 0 && d.logprob) {
+    lab = d.labels[r];
+    if (lab >= 0) xl = static_cast<uint32_t>(lab) < V ? Ty<T>::to(sh.x[lab]) : nan_f();
   }
-  for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
-    const Key e = lists[i];
-    if (e == 0) continue;                              // fewer than K of the block's elements reach the bound
-    const uint32_t own = i / K;
-    uint32_t ahead = i - own * K;
-    for (uint32_t b = 0; b < blocks; ++b)
-      if (b != own) ahead += count_above(lists + b * K, K, e);
-    if (ahead < K) {
-      d.top_id[r * K + ahead] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
-      d.top_logprob[r * K + ahead] = logprob(key_value(e));
-    }
+  const float c = kLog2e / d.temperature;
+  const Stats a = stream_stats<T, ENT>(sh, c, nullptr);
+  const float wmax = warp_max_nan(a.m);
+  if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
+  const uint32_t key = threadIdx.x < sh.n ? order_key(a.m) : 0u;
+  ts.key[threadIdx.x] = key;
+  __syncthreads();
+  const float m = block_max(ss);
+  join_threads<ENT>(ss, a, c, m);
+  if (K && first_warp) {
+    const uint32_t bound = top_bound(ts, sh.n, K);
+    if (threadIdx.x == 0) ts.bound[0] = bound;
   }
+  __syncthreads();
+  if (first_warp) send_block_stats(ss, m, cl, 0, 1, 1);
+  if (K) block_top(sh, [&](uint32_t i) { return row_vec(sh, i); }, key, ts.bound[0], K, ts, list);
+  __syncthreads();
+  write_scores(d, r, ss.block[0], lab, xl, list, 1);
 }
 
 // ---- gradient of the scores ----------------------------------------------------------------------
@@ -737,6 +922,99 @@ __device__ __forceinline__ void distill_factors(TeacherShared& th, uint32_t K, b
   th.inv_z = tail ? 1.0 : z == 0.0 ? 0.0 : 1.0 / z;
 }
 
+// Sum of the student's exponentials over all tokens, at the row's maximum m, from that over the unnamed ones.
+__device__ __forceinline__ float student_sum(const TeacherShared& th, uint32_t K, const Stats& row, float base, float m,
+                                             double log2e_t) {
+  const float es = static_cast<float>(entry_sum(th.s, K));
+  float S = 0.0f;
+  if (row.s != 0.0f) S = row.s * exp_of(row.m - m, log2e_t);
+  if (es != 0.0f) S += es * exp_of(base - m, log2e_t);
+  return m != m ? nan_f() : S;
+}
+// Entry of this thread: what does not wait for anything.
+__device__ __forceinline__ Entry load_entry(const seeml_b200_distill_topk& d, size_t r) {
+  Entry e{-1, false, -INFINITY, -INFINITY, 0.0, 0.0};
+  if (threadIdx.x < d.top_k) {
+    e.id = d.teacher_id[r * d.top_k + threadIdx.x];
+    const float v = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * d.top_k + threadIdx.x);
+    if (e.id >= 0) e.v = v;
+  }
+  return e;
+}
+__device__ __forceinline__ void publish_entries(uint32_t K, TeacherShared& th, const Entry& e) {
+  if (threadIdx.x == 0) th.bad = th.dup = 0;
+  if (!entry_warp(K)) return;
+  th.id[threadIdx.x] = e.id;
+  const float vm = warp_max_nan(e.v), xm = warp_max_nan(e.x);
+  if ((threadIdx.x & 31) == 0) { th.v[threadIdx.x >> 5] = vm; th.x[threadIdx.x >> 5] = xm; }
+}
+// The loss of a row, and what a backward call needs: by one block, behind the gradient that nobody waits for.
+__device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, TeacherShared& th, const Stats& row, const Entry& e,
+                                             float base) {
+  const seeml_b200_distill_topk& d = a.d;
+  const uint32_t K = d.top_k;
+  const bool tail = d.tail != 0;
+  const double z = entry_sum(th.z, K), log_z = ln_sum(static_cast<float>(z));
+  if (entry_warp(K)) {                       // sum of q (ln q - (x - base) / T)
+    double l = 0.0;
+    if (e.q != 0.0) {
+      const double log_q = tail ? e.v : static_cast<double>(e.v) - entry_max(th.v, K) - log_z;
+      l = e.x == -INFINITY ? INFINITY : (tail ? e.q : e.q / z) * (log_q - (static_cast<double>(e.x) - base) * a.inv_t);
+    }
+    l = warp_sum(l);
+    if ((threadIdx.x & 31) == 0) th.l[threadIdx.x >> 5] = l;
+  }
+  if (K > 32) __syncthreads();
+  if (threadIdx.x != 0) return;
+  const float m = max_nan(row.m, base), st = row.s, S = student_sum(th, K, row, base, m, a.log2e_t);
+  double qsum, rest;
+  teacher_mass(z, tail, qsum, rest);
+  const double log_s = ln_sum(S);
+  double l = entry_sum(th.l, K);
+  if (qsum != 0.0) l += qsum * ((static_cast<double>(m) - base) * a.inv_t + log_s);
+  if (qsum != 0.0 && S == 0.0f) l = INFINITY;
+  if (rest > 0.0 && st != 0.0f)
+    l += rest * (log(rest) - ((static_cast<double>(row.m) - m) * a.inv_t + ln_sum(st) - log_s));
+  d.row_loss[r] = th.bad ? nan_f() : static_cast<float>(l);
+  if (d.saved) {
+    float* sv = d.saved + 4 * r;
+    sv[0] = row.m; sv[1] = st; sv[2] = m; sv[3] = S;
+  }
+}
+// A row of weight 0, or this block's share of it.
+template <class T>
+__device__ __forceinline__ void skip_row(const DistillArgs& a, size_t r, const Share<T>& sh, T* g, bool same, bool loss) {
+  const seeml_b200_distill_topk& d = a.d;
+  if (g) {
+    float2 f[Ty<T>::E / 2];
+#pragma unroll
+    for (int q = 0; q < Ty<T>::E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
+    for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
+      const int j = sh.elem(i);
+      if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + j) = make_uint4(0, 0, 0, 0);
+      else store_elems<T>(g, j, sh.V, f);
+    }
+  }
+  if (loss && threadIdx.x == 0) {
+    d.row_loss[r] = 0.0f;
+    if (d.saved) {
+      float* sv = d.saved + 4 * r;
+      sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;
+    }
+  }
+}
+// A named token's gradient, over what the sweep of its block left there (behind a barrier).
+template <class T>
+__device__ __forceinline__ void store_named(T* g, uint32_t K, const TeacherShared& th, const Entry& e, float up_t) {
+  double q = e.q;
+  if (th.dup) {
+    q = 0.0;
+    for (uint32_t j = 0; j < K; ++j)
+      if (th.id[j] == e.id) q += th.q[j];
+  }
+  g[e.id] = Ty<T>::from(th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named - q * th.inv_z)));
+}
+
 template <class T, int MODE>
 __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32_t share, uint32_t blocks) {
   constexpr int E = Ty<T>::E;
@@ -754,30 +1032,9 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
   const bool same = MODE != kLoss && (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
   // the row's weight and its entries arrive together; the row is only asked for if it counts
   const float w = MODE == kBackward ? a.upstream[r] : d.row_weight ? d.row_weight[r] : 1.0f;
-  Entry e{-1, false, -INFINITY, -INFINITY, 0.0, 0.0};
-  if (threadIdx.x < K) {
-    e.id = d.teacher_id[r * K + threadIdx.x];
-    const float v = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * K + threadIdx.x);
-    if (e.id >= 0) e.v = v;
-  }
+  Entry e = load_entry(d, r);
   if (w == 0.0f) {                                     // the whole cluster leaves here
-    if (MODE != kLoss) {
-      float2 f[E / 2];
-#pragma unroll
-      for (int q = 0; q < E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
-      for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) {
-        const int j = sh.elem(i);
-        if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + j) = make_uint4(0, 0, 0, 0);
-        else store_elems<T>(g, j, V, f);
-      }
-    }
-    if (MODE != kBackward && rank == 0 && threadIdx.x == 0) {
-      d.row_loss[r] = 0.0f;
-      if (d.saved) {
-        float* sv = d.saved + 4 * r;
-        sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;
-      }
-    }
+    skip_row(a, r, sh, g, same, MODE != kBackward && rank == 0);
     return;
   }
   sh.load(sm);
@@ -786,12 +1043,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
   // Read here, ahead of the cluster's barrier: in place, another block may overwrite it behind that. The backward
   // call has no such barrier and needs only the entries of its own share, which it finds in shared memory.
   if (MODE != kBackward && e.id >= 0 && static_cast<uint32_t>(e.id) < V) e.x = Ty<T>::to(sh.x[e.id]);
-  if (threadIdx.x == 0) th.bad = th.dup = 0;
-  if (entries) {
-    th.id[threadIdx.x] = e.id;
-    const float vm = warp_max_nan(e.v), xm = warp_max_nan(e.x);
-    if ((threadIdx.x & 31) == 0) { th.v[threadIdx.x >> 5] = vm; th.x[threadIdx.x >> 5] = xm; }
-  }
+  publish_entries(K, th, e);
   __syncthreads();
   const float base = MODE == kBackward ? 0.0f : entry_max(th.x, K);
   if (entries) entries_exp(V, K, tail, a.inv_t, base, th, e);
@@ -829,11 +1081,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
     if (MODE == kStep) {
       if (threadIdx.x == 0) {
         const Stats row = row_stats(ss, c, blocks);
-        const float m = max_nan(row.m, base), es = static_cast<float>(entry_sum(th.s, K));
-        float S = 0.0f;
-        if (row.s != 0.0f) S = row.s * exp_of(row.m - m, a.log2e_t);
-        if (es != 0.0f) S += es * exp_of(base - m, a.log2e_t);
-        if (m != m) S = nan_f();
+        const float m = max_nan(row.m, base), S = student_sum(th, K, row, base, m, a.log2e_t);
         distill_factors(th, K, tail, up_t, row.m, row.s, m, S, base, a.log2e_t);
       }
       __syncthreads();
@@ -876,51 +1124,92 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(DistillArgs a, uint32
       }
     }
     __syncthreads();
-    if (at >= 0 && e.first) {
-      double q = e.q;
-      if (th.dup) {
-        q = 0.0;
-        for (uint32_t j = 0; j < K; ++j)
-          if (th.id[j] == e.id) q += th.q[j];
-      }
-      g[e.id] = Ty<T>::from(th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named - q * th.inv_z)));
-    }
+    if (at >= 0 && e.first) store_named(g, K, th, e, up_t);
   }
-  // the loss, behind the gradient that nobody waits for: sum of q (ln q - (x - base) / T) over the entries first
-  if (MODE != kBackward && rank == 0) {
-    const double z = entry_sum(th.z, K), log_z = ln_sum(static_cast<float>(z));
-    if (entries) {
-      double l = 0.0;
-      if (e.q != 0.0) {
-        const double log_q = tail ? e.v : static_cast<double>(e.v) - entry_max(th.v, K) - log_z;
-        l = e.x == -INFINITY ? INFINITY : (tail ? e.q : e.q / z) * (log_q - (static_cast<double>(e.x) - base) * a.inv_t);
-      }
-      l = warp_sum(l);
-      if ((threadIdx.x & 31) == 0) th.l[threadIdx.x >> 5] = l;
-    }
-    if (K > 32) __syncthreads();
+  if (MODE != kBackward && rank == 0) distill_loss(a, r, th, row_stats(ss, c, blocks), e, base);
+}
+
+// Loss and gradient of a row that one block streams: twice, the second time out of L2 (the rows of all blocks in
+// flight fit there). Named tokens are left out of the sums by a byte per vector.
+template <class T, int MODE>
+__global__ void __launch_bounds__(kThreads, 4) distill_stream_kernel(DistillArgs a) {
+  constexpr int E = Ty<T>::E;
+  extern __shared__ uint32_t named[];
+  __shared__ TeacherShared th;
+  __shared__ StatsShared ss;
+  const seeml_b200_distill_topk& d = a.d;
+  cg::cluster_group cl = cg::this_cluster();
+  const size_t r = blockIdx.x;
+  const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  const bool tail = d.tail != 0, first_warp = threadIdx.x < 32, entries = entry_warp(K);
+  const Share<T> sh(d.logits, r, d.row_stride, V, 1, 0);
+  T* g = MODE == kStep ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
+  const bool same = MODE == kStep && (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
+  const float w = d.row_weight ? d.row_weight[r] : 1.0f;
+  Entry e = load_entry(d, r);
+  if (w == 0.0f) {
+    skip_row(a, r, sh, g, same, true);
+    return;
+  }
+  const uint32_t batches = (sh.n + kBatchVecs - 1) / kBatchVecs;
+  for (uint32_t i = threadIdx.x; i < batches * kThreads; i += kThreads) named[i] = 0;
+  const bool there = e.id >= 0 && static_cast<uint32_t>(e.id) < V;
+  if (there) e.x = Ty<T>::to(sh.x[e.id]);
+  publish_entries(K, th, e);
+  __syncthreads();
+  const float base = entry_max(th.x, K);
+  if (there) {
+    const uint32_t p = static_cast<uint32_t>(e.id) + sh.phase, i = p / E;
+    atomicOr(&named[i / kBatchVecs * kThreads + i % kThreads], 1u << (i % kBatchVecs / kThreads * 8 + p % E));
+  }
+  if (entries) entries_exp(V, K, tail, a.inv_t, base, th, e);
+  __syncthreads();
+  const float c = kLog2e / d.temperature;
+  const Stats mine = stream_stats<T, false>(sh, c, named);
+  const float wmax = warp_max_nan(mine.m);
+  if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
+  __syncthreads();
+  const float bm = block_max(ss);
+  join_threads<false>(ss, mine, c, bm);
+  __syncthreads();
+  if (first_warp) send_block_stats(ss, bm, cl, 0, 1, 1);
+  if (MODE == kStep) {
+    const float up_t = d.scale * w / d.temperature;
+    uint4 v[kBatch];
+    row_batch(sh, 0, v);
     if (threadIdx.x == 0) {
-      const Stats row = row_stats(ss, c, blocks);
-      const float m = max_nan(row.m, base), st = row.s, es = static_cast<float>(entry_sum(th.s, K));
-      float S = 0.0f;
-      if (st != 0.0f) S = st * exp_of(row.m - m, a.log2e_t);
-      if (es != 0.0f) S += es * exp_of(base - m, a.log2e_t);
-      if (m != m) S = nan_f();
-      double qsum, rest;
-      teacher_mass(z, tail, qsum, rest);
-      const double log_s = ln_sum(S);
-      double l = entry_sum(th.l, K);
-      if (qsum != 0.0) l += qsum * ((static_cast<double>(m) - base) * a.inv_t + log_s);
-      if (qsum != 0.0 && S == 0.0f) l = INFINITY;
-      if (rest > 0.0 && st != 0.0f)
-        l += rest * (log(rest) - ((static_cast<double>(row.m) - m) * a.inv_t + ln_sum(st) - log_s));
-      d.row_loss[r] = bad ? nan_f() : static_cast<float>(l);
-      if (d.saved) {
-        float* sv = d.saved + 4 * r;
-        sv[0] = row.m; sv[1] = st; sv[2] = m; sv[3] = S;
+      const Stats row = ss.block[0];
+      const float m = max_nan(row.m, base);
+      distill_factors(th, K, tail, up_t, row.m, row.s, m, student_sum(th, K, row, base, m, a.log2e_t), base, a.log2e_t);
+    }
+    __syncthreads();
+    const float2 shift = make_float2(-th.mt, -th.mt), c2 = make_float2(c, c), A2 = make_float2(th.A, th.A);
+    for (uint32_t b = 0; b < batches; ++b) {
+      uint4 next[kBatch];
+      if (b + 1 < batches) row_batch(sh, b + 1, next);
+      const bool whole = same && b * kBatchVecs >= sh.lo && (b + 1) * kBatchVecs <= sh.hi;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const uint32_t i = b * kBatchVecs + u * kThreads + threadIdx.x;
+        const int j = sh.elem(i);
+        float2 f[E / 2];
+        Ty<T>::unpack(v[u], f);
+#pragma unroll
+        for (int q = 0; q < E / 2; ++q) {
+          const float2 y = mul2(add2(f[q], shift), c2);
+          f[q] = mul2(make_float2(ex2(y.x), ex2(y.y)), A2);
+        }
+        if (whole || (same && sh.whole(i))) *reinterpret_cast<uint4*>(g + j) = Ty<T>::pack(f);
+        else if (i < sh.n) store_elems<T>(g, j, V, f);
+        v[u] = next[u];
       }
     }
+    __syncthreads();
+    if (there && e.first && !th.bad) store_named(g, K, th, e, up_t);
+  } else {
+    __syncwarp();
   }
+  distill_loss(a, r, th, ss.block[0], e, base);
 }
 
 // loss = scale * sum of weight * row_loss, in a fixed order and 64 bits: one block, four rows in flight per thread.
@@ -954,6 +1243,7 @@ int by_type(uint32_t dtype, F f) {
 // Blocks per row. A share of at most 66 KiB lets three blocks live on an SM, so that one copies
 // while others compute; a call of few rows is spread further, down to 8 KiB a block, until it
 // covers the SMs.
+constexpr uint64_t kStreamRows = 2 * kSMs;
 struct Split {
   uint32_t blocks, share;      // share in 16-byte vectors
 };
@@ -993,11 +1283,26 @@ int launch_rows(uint64_t rows, const Split& s, bool cluster, size_t lists, cudaS
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, Kernel, args..., s.share, s.blocks) == cudaSuccess ? 1 : -1;
 }
+template <auto Kernel, class... Args>
+int launch_stream(uint64_t rows, size_t smem, cudaStream_t st, Args... args) {
+  static std::atomic<uint64_t> done{0};
+  if (smem > (40u << 10) && !allow_smem(Kernel, done)) return -1;
+  Kernel<<<static_cast<unsigned>(rows), kThreads, smem, st>>>(args...);
+  return 1;
+}
+bool streams(uint64_t rows, uint64_t) { return rows >= kStreamRows; }
 uint64_t elem_bytes(uint32_t dtype) { return dtype == SEEML_B200_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace
 
 int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
+  if (streams(d.rows, d.vocab))
+    return by_type(d.dtype, [&](auto t) {
+      using T = decltype(t);
+      if (d.entropy) token_scores_stream_kernel<T, true><<<static_cast<unsigned>(d.rows), kThreads, 0, st>>>(d);
+      else token_scores_stream_kernel<T, false><<<static_cast<unsigned>(d.rows), kThreads, 0, st>>>(d);
+      return 1;
+    });
   const Split s = split_row(d.rows, d.vocab, elem_bytes(d.dtype));
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
@@ -1021,8 +1326,17 @@ static DistillArgs distill_args(const seeml_b200_distill_topk& d) {
   return DistillArgs{d, nullptr, nullptr, inv_t, inv_t / kLn2};
 }
 int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
-  const Split s = split_row(d.rows, d.vocab, elem_bytes(d.dtype));
   const DistillArgs a = distill_args(d);
+  if (streams(d.rows, d.vocab)) {
+    const uint64_t per = 16 / elem_bytes(d.dtype), vecs = (d.vocab + 2 * (per - 1)) / per;
+    const Split s{1, static_cast<uint32_t>((vecs + kBatchVecs - 1) / kBatchVecs * kThreads / 4)};      // a word per batch and thread
+    return by_type(d.dtype, [&](auto t) {
+      using T = decltype(t);
+      return d.dlogits ? launch_stream<distill_stream_kernel<T, kStep>>(d.rows, s.share * 16, st, a)
+                       : launch_stream<distill_stream_kernel<T, kLoss>>(d.rows, s.share * 16, st, a);
+    });
+  }
+  const Split s = split_row(d.rows, d.vocab, elem_bytes(d.dtype));
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
     return d.dlogits ? launch_rows<distill_kernel<T, kStep>>(d.rows, s, true, 0, st, a)

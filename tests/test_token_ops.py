@@ -131,11 +131,32 @@ def _close(got, want, bound, dtype, what):
     assert not bad.any(), f"{what}: {bad.sum()} of {bad.size} out; worst {np.max(err / bar):.3f} of the bound"
 
 
+def _copies(result, rows):
+    """Results of a call whose rows repeat, by copy. A row's bits depend on how it lies in the 16-byte vectors of memory,
+    which repeats after 8 copies at the latest: those are returned, the others have to equal them."""
+    period = 8 * rows
+    out = []
+    for c in range(min(8, result[1].shape[0] // rows)):
+        part = []
+        for t in result:
+            if t is not None and t.dim():
+                mine = torch.cat([t[r:r + rows] for r in range(c * rows, t.shape[0], period)])
+                bits = mine.reshape(-1, rows, mine[0].numel()).contiguous().view(torch.uint8)
+                assert torch.equal(bits, bits[:1].expand(bits.shape[0], -1, -1))
+                t = t[c * rows:(c + 1) * rows]
+            part.append(t)
+        out.append(type(result)(*part))
+    return out
+
+
 SHAPES = [  # rows, vocab, dtype, pad, temperature, masked
     (1, 1, F32, 0, 1.0, 0.0), (3, 2, F16, 1, 0.5, 0.0), (5, 7, BF16, 0, 1.0, 0.3), (2, 33, F32, 3, 2.0, 0.5),
     (9, 255, F16, 0, 1.0, 0.0), (4, 1000, F32, 0, 0.7, 0.9), (3, 4097, BF16, 5, 1.5, 0.2), (1, 5000, F32, 0, 1.0, 0.0),
     (300, 513, F32, 0, 1.0, 0.1), (7, 32000, F32, 0, 1.0, 0.0), (2, 32000, BF16, 0, 0.8, 0.3), (5, 50001, F16, 7, 1.0, 0.0),
-    (1, 131072, BF16, 0, 1.0, 0.0), (3, 100003, F32, 0, 2.0, 0.6), (2, 393216, F32, 0, 1.0, 0.0), (1, 786432, F16, 0, 1.0, 0.0)]
+    (1, 131072, BF16, 0, 1.0, 0.0), (3, 100003, F32, 0, 2.0, 0.6), (2, 393216, F32, 0, 1.0, 0.0), (1, 786432, F16, 0, 1.0, 0.0),
+    # calls of many rows, which give each row to one block
+    (300, 1, F32, 0, 1.0, 0.0), (301, 11, BF16, 2, 1.0, 0.2), (400, 1027, F16, 0, 0.6, 0.4), (300, 9001, F32, 3, 1.0, 0.0),
+    (297, 20001, BF16, 0, 1.5, 0.3), (310, 16384, F16, 8, 1.0, 0.0)]
 
 
 def _ids(v):
@@ -165,8 +186,9 @@ def test_token_scores(backend_lib, rows, V, dtype, pad, T, masked, k):
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=_ids)
 @pytest.mark.parametrize("V,k", [(40, 40), (3000, 17), (32000, 128), (100003, 100)])
+@pytest.mark.parametrize("copies", [1, 160])
 @pytest.mark.parametrize("shape", ["constant", "ascending", "descending", "few", "one_slice", "zeros_of_both_signs", "lowest"])
-def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape):
+def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape, copies):
     """Ties go to the lower index, whatever the order and wherever the great values lie."""
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(V + k)
@@ -175,16 +197,17 @@ def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape):
          "one_slice": np.where((j // 8) % 512 == 3, 5.0 + rng.standard_normal(V), rng.standard_normal(V)),
          "zeros_of_both_signs": np.where(j % 2, 0.0, -0.0), "lowest": np.full(V, torch.finfo(dtype).min)}[shape]
     t = torch.from_numpy(np.stack([x, x[::-1].copy()])).to(dtype).cuda()
-    s = ops.token_scores(t, None, top_k=k)
     _, h, tlp, tid = R.scores(_f64(t), None, k, 1.0)
-    np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
-    _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
-    _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
+    for s in _copies(ops.token_scores(t.repeat(copies, 1), None, top_k=k), 2):
+        np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+        _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
+        _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
 
 
 @gpu
+@pytest.mark.parametrize("copies", [1, 43])
 @pytest.mark.parametrize("V", [5, 700, 32000])
-def test_rows_that_are_masked_or_not_finite(backend_lib, V):
+def test_rows_that_are_masked_or_not_finite(backend_lib, V, copies):
     from see_ml_b200 import token_ops as ops
     x = np.random.default_rng(V).standard_normal((7, V))
     x[0] = -np.inf                           # nothing left
@@ -196,12 +219,13 @@ def test_rows_that_are_masked_or_not_finite(backend_lib, V):
     x[5, 4] = np.nan
     t = torch.from_numpy(x).float().cuda()
     labels = np.array([1, 0, 0, 0, 1, 3, V + 5], np.int32)
-    s = ops.token_scores(t, torch.from_numpy(labels).cuda(), top_k=4, temperature=0.5, stats=True)
     lp, h, tlp, tid = R.scores(_f64(t), labels, 4, 0.5)
-    np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
-    _close(s.logprob, lp, R.delta(V), F32, "logprob")
-    _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
-    _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
+    for s in _copies(ops.token_scores(t.repeat(copies, 1), torch.from_numpy(labels).cuda().repeat(copies), top_k=4,
+                                      temperature=0.5, stats=True), 7):
+        np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+        _close(s.logprob, lp, R.delta(V), F32, "logprob")
+        _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
+        _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
     ones = torch.ones(7, device="cuda")
     g = _f64(ops.token_scores_backward(t, torch.from_numpy(labels).cuda(), s.stats, s.entropy, ones, ones, temperature=0.5))
     assert (g[0] == 0).all() and np.isnan(g[1]).all() and np.isnan(g[2]).all() and np.isnan(g[6]).all()
@@ -272,9 +296,10 @@ def test_distill(backend_lib, rows, V, dtype, pad, T, masked, K, tail, tdtype):
 
 
 @gpu
+@pytest.mark.parametrize("copies", [1, 30])
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("V", [9, 3000, 70001])
-def test_distill_of_awkward_rows(backend_lib, V, tail):
+def test_distill_of_awkward_rows(backend_lib, V, tail, copies):
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(V)
     x = rng.standard_normal((10, V)) * 2
@@ -295,23 +320,28 @@ def test_distill_of_awkward_rows(backend_lib, V, tail):
     vt = torch.from_numpy(v).float().cuda()
     it = torch.from_numpy(ids).cuda()
     good = [i for i in range(10) if i != 7]
-    for out in (None, t.clone()):
-        src = t if out is None else out
-        r = ops.distill_topk(src, it, vt, tail=tail, grad=True, saved=True, out=out)
+    for out in (None, t.repeat(copies, 1)):
+        src = t.repeat(copies, 1) if out is None else out
         loss, lerr, grad, gerr = R.distill(_f64(t)[good], ids[good], _f64(vt)[good], 1.0, tail)
-        _close(r.row_loss[good], loss, lerr, F32, "row_loss")
-        _close(r.dlogits[good], grad, gerr, F32, "dlogits")
-        assert torch.isnan(r.row_loss[7]) and torch.isnan(r.dlogits[7]).all()
-    g = ops.distill_topk_backward(t, it, vt, r.saved, torch.ones(10, device="cuda"), tail=tail)
+        for r in _copies(ops.distill_topk(src, it.repeat(copies, 1), vt.repeat(copies, 1), tail=tail, grad=True, saved=True,
+                                          out=out), 10):
+            _close(r.row_loss[good], loss, lerr, F32, "row_loss")
+            _close(r.dlogits[good], grad, gerr, F32, "dlogits")
+            assert torch.isnan(r.row_loss[7]) and torch.isnan(r.dlogits[7]).all()
+    g = ops.distill_topk_backward(t, it, vt, r.saved.contiguous(), torch.ones(10, device="cuda"), tail=tail)
     _close(g[good], grad, gerr, F32, "dlogits of the backward call")
     assert torch.isnan(g[7]).all()
     x[5, 0] = np.nan                  # a row of weight 0 is not looked at, another is
     t = torch.from_numpy(x).float().cuda()
     w = torch.ones(10, device="cuda")
-    r = ops.distill_topk(t, it, vt, tail=tail, grad=True, row_weight=w)
+
+    def weighted():
+        return _copies(ops.distill_topk(t.repeat(copies, 1), it.repeat(copies, 1), vt.repeat(copies, 1), tail=tail, grad=True,
+                                        row_weight=w.repeat(copies)), 10)[0]
+    r = weighted()
     assert torch.isnan(r.row_loss[5]) and torch.isnan(r.dlogits[5]).all() and torch.isnan(r.loss)
     w[5] = w[6] = w[7] = 0.0
-    r = ops.distill_topk(t, it, vt, tail=tail, grad=True, row_weight=w)
+    r = weighted()
     assert (r.row_loss[5:8] == 0).all() and (r.dlogits[5:8] == 0).all() and torch.isfinite(r.loss)
 
 
@@ -342,12 +372,12 @@ def test_gradients_against_differences(backend_lib, tail):
 
 @gpu
 @pytest.mark.parametrize("dtype,V", [(BF16, 4097), (F32, 1000), (F16, 32001)], ids=_ids)
+@pytest.mark.parametrize("rows", [5, 300])
 @pytest.mark.parametrize("xo,go,xs,gs", [(0, 0, 0, 0), (1, 0, 3, 0), (0, 5, 0, 8), (3, 3, 7, 7), (8, 2, 1, 9)])
-def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs):
+def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs, rows):
     """Rows that start anywhere, gradients whose rows start elsewhere; nothing beside them is touched."""
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(V + xo)
-    rows = 5
     xb = torch.zeros(16 + rows * (V + xs), dtype=dtype, device="cuda")
     x = xb[xo:xo + rows * (V + xs)].view(rows, V + xs)[:, :V]
     x.copy_(torch.from_numpy(rng.standard_normal((rows, V)) * 2))
@@ -430,11 +460,12 @@ def test_device_refusals(backend_lib):
 
 
 @gpu
-def test_streams_and_graphs_give_the_same_bits(backend_lib):
+@pytest.mark.parametrize("rows", [40, 320])
+def test_streams_and_graphs_give_the_same_bits(backend_lib, rows):
     """The calls of a step on two streams at once and in two captured graphs: no scratch is shared."""
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(1)
-    rows, V, k = 40, 20011, 24
+    V, k = 20011, 24
     xs = [torch.from_numpy(rng.standard_normal((rows, V)) * 2).to(BF16).cuda() for _ in range(2)]
     lab = torch.arange(rows, dtype=torch.int32, device="cuda")
     one = torch.ones(rows, device="cuda")
