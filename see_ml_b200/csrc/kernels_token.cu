@@ -410,11 +410,14 @@ __device__ __forceinline__ void batch_sums(const uint4 (&v)[kBatch], float shift
   }
 }
 // Statistics of this thread's vectors of the row, in one pass with a running maximum. named: a byte per vector whose
-// bits are the elements to leave out, the bytes of a thread's batch in one word (NULL: none).
+// bits are the elements to leave out, the bytes of a thread's batch in one word (NULL: none). runs: [run][thread] gets
+// the maximum of every per_run batches (NULL: not wanted).
 template <class T, bool ENT>
-__device__ __forceinline__ Stats stream_stats(const Share<T>& sh, float c, const uint32_t* named) {
+__device__ __forceinline__ Stats stream_stats(const Share<T>& sh, float c, const uint32_t* named, float* runs, uint32_t per_run) {
   Stats a{-INFINITY, 0.0f, 0.0f};
   const uint32_t batches = (sh.n + kBatchVecs - 1) / kBatchVecs;
+  float run = -INFINITY;
+  uint32_t left = per_run;
   uint4 v[kBatch];
   row_batch(sh, 0, v);
   for (uint32_t b = 0; b < batches; ++b) {
@@ -431,6 +434,15 @@ __device__ __forceinline__ Stats stream_stats(const Share<T>& sh, float c, const
     float m = Ty<T>::vmax(v[0]);
 #pragma unroll
     for (int u = 1; u < kBatch; ++u) m = max_nan(m, Ty<T>::vmax(v[u]));
+    if (runs) {
+      run = max_nan(run, m);
+      if (--left == 0 || b + 1 == batches) {
+        runs[threadIdx.x] = run;
+        runs += kThreads;
+        run = -INFINITY;
+        left = per_run;
+      }
+    }
     m = max_nan(m, a.m);
     const float shift = m == -INFINITY ? 0.0f : m;
     float s, t = 0.0f;
@@ -471,12 +483,16 @@ __device__ __forceinline__ float key_value(Key key) {
   return k == 0xffffffffu ? nan_f() : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 constexpr int kCand = 512;                  // candidates of a block's selection
+constexpr int kHot = 1024;                  // runs of vectors that it looks at again
+constexpr int kSegs = 16;                   // runs of a thread's vectors whose maxima are kept
 struct TopShared {
   __align__(16) Key cand[kCand];
   uint32_t key[kThreads];
-  uint16_t hot[kThreads];
+  uint16_t hot[kHot];                       // thread | run << 8
+  uint32_t warp[kWarps];
   uint32_t bound[kClusterMax], hots, count;
 };
+static_assert(kThreads <= 256, "a hot run's code holds the thread in 8 bits");
 // Calls f(key) for the elements of vector i whose key is at least `least` (thr: the value of that key).
 template <class T, class F>
 __device__ __forceinline__ void each_from(const Share<T>& sh, const uint4& vec, uint32_t i, uint32_t least, float thr, F f) {
@@ -523,61 +539,130 @@ __device__ __forceinline__ uint32_t top_bound(const TopShared& ts, uint32_t n, u
   }
   return lo;
 }
-// The block's elements that reach the bound, best first, into out[0 .. k): at most k, then zeros. Only the vectors of
-// threads whose maximum reaches the bound are looked at again (vec(i) brings vector i), by all warps; what they hold
-// is ranked by counting.
-// ts.hots and ts.count are zero ahead of the barrier that the caller passed last.
+// Where a block's vectors are found again: in its shared memory, or in the row.
+struct ParkedVecs {
+  const uint4* sm;
+  template <class T> __device__ __forceinline__ uint4 operator()(const Share<T>&, uint32_t i) const { return sm[i]; }
+};
+struct RowVecs {
+  template <class T> __device__ __forceinline__ uint4 operator()(const Share<T>& sh, uint32_t i) const { return row_vec(sh, i); }
+};
+// Counts the block's elements whose key is at least `least`. Every thread gets the result.
 template <class T, class Vec>
-__device__ __forceinline__ void block_top(const Share<T>& sh, Vec vec, uint32_t key, uint32_t bound, uint32_t k, TopShared& ts,
-                                          Key* out) {
+__device__ __forceinline__ uint32_t count_from(const Share<T>& sh, Vec vec, uint32_t least, TopShared& ts) {
+  const float thr = key_value(static_cast<Key>(least) << 32);
+  uint32_t mine = 0;
+  for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads) each_from(sh, vec(sh, i), i, least, thr, [&](Key) { ++mine; });
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) ts.warp[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  mine = 0;
+  for (int w = 0; w < kWarps; ++w) mine += ts.warp[w];
+  return mine;
+}
+// What block_top does when more than kCand elements reach its bound, or more than kHot runs: sorted rows, rows of few
+// different values. The bound is raised until it fits, or is the k-th value itself; then the elements above it come
+// first and those equal to it fill up by their index, which is where they lie. Returns how many are in ts.cand.
+template <class T, class Vec>
+__device__ __noinline__ uint32_t top_overflow(const T* x, uint32_t V, uint32_t blocks, uint32_t rank, Vec vec, uint32_t lo,
+                                              uint32_t k, TopShared& ts) {
+  const Share<T> sh(x, 0, 0, V, blocks, rank);
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t hi = 0;
+  for (int q = 0; q < kThreads; ++q) hi = max(hi, ts.key[q]);
+  uint32_t at = ~0u;                                     // elements that reach lo, once known
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    const uint32_t c = count_from(sh, vec, mid, ts);
+    if (c >= k) lo = mid, at = c;
+    else hi = mid - 1;
+    if (c >= k && c <= kCand) break;
+  }
+  const bool fits = at <= kCand;
+  const uint32_t least = fits ? lo : lo + 1;             // lo is below 0xffffffff unless there are k NaNs
+  __syncthreads();
+  if (threadIdx.x == 0) ts.count = 0;
+  __syncthreads();
+  if (least > lo || fits) {
+    const float thr = key_value(static_cast<Key>(least) << 32);
+    for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
+      each_from(sh, vec(sh, i), i, least, thr, [&](Key e) { ts.cand[atomicAdd(&ts.count, 1u)] = e; });
+  }
+  __syncthreads();
+  uint32_t have = ts.count;                              // fits: at; else fewer than k
+  const float thr = key_value(static_cast<Key>(lo) << 32);
+  for (uint32_t first = 0; !fits && first < sh.n && have < k; first += kThreads) {
+    const uint32_t i = first + threadIdx.x;
+    uint32_t mine = 0;
+    auto equal = [&](auto f) {
+      if (i < sh.n) each_from(sh, vec(sh, i), i, lo, thr, [&](Key e) { if (static_cast<uint32_t>(e >> 32) == lo) f(e); });
+    };
+    equal([&](Key) { ++mine; });
+    uint32_t upto = mine;                                // threads are in the order of their vectors
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t p = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += p;
+    }
+    __syncthreads();
+    if (lane == 31) ts.warp[warp] = upto;
+    __syncthreads();
+    uint32_t pos = have + upto - mine, all = 0;
+    for (uint32_t w = 0; w < kWarps; ++w) {
+      if (w < warp) pos += ts.warp[w];
+      all += ts.warp[w];
+    }
+    equal([&](Key e) {
+      if (pos < k) ts.cand[pos] = e;
+      ++pos;
+    });
+    have = min(have + all, k);
+  }
+  __syncthreads();
+  return have;
+}
+// The block's elements that reach the bound, best first, into out[0 .. k): at most k, then zeros. Only the runs of
+// vectors whose maximum reaches the bound are looked at again, by all warps; what they hold
+// is ranked by counting. runs: maxima [run][thread] of `len` vectors each (NULL: one run per thread, all its vectors,
+// and key is its maximum's). ts.hots and ts.count are zero ahead of the barrier that the caller passed last.
+template <class T, class Vec>
+__device__ __forceinline__ void block_top(const Share<T>& sh, uint32_t blocks, uint32_t rank, Vec vec, uint32_t key, uint32_t bound, uint32_t k, TopShared& ts,
+                                          Key* out, const float* runs, uint32_t n_runs, uint32_t len) {
   const uint32_t lane = threadIdx.x & 31;
-  if (threadIdx.x < sh.n && key >= bound) ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
+  if (threadIdx.x < sh.n && key >= bound) {
+    if (!runs) {
+      ts.hot[atomicAdd(&ts.hots, 1u)] = static_cast<uint16_t>(threadIdx.x);
+    } else {
+      for (uint32_t q = 0; q < n_runs; ++q)
+        if (order_key(runs[q * kThreads + threadIdx.x]) >= bound) {
+          const uint32_t p = atomicAdd(&ts.hots, 1u);
+          if (p < kHot) ts.hot[p] = static_cast<uint16_t>(threadIdx.x | q << 8);
+        }
+    }
+  }
   __syncthreads();
   const float thr = bound == 0 ? -INFINITY : key_value(static_cast<Key>(bound) << 32);
-  {
-    // a thread's vectors by as many lanes as it has vectors (a power of two, 32 at most)
-    const uint32_t hots = ts.hots, per_thread = (sh.n + kThreads - 1) / kThreads;
-    const uint32_t wide = per_thread > 16 ? 5u : per_thread > 8 ? 4u : per_thread > 4 ? 3u : per_thread > 2 ? 2u : per_thread > 1 ? 1u : 0u;
-    for (uint32_t h = threadIdx.x >> wide; h < hots; h += kThreads >> wide)
-      for (uint32_t i = ts.hot[h] + (lane & ((1u << wide) - 1)) * kThreads; i < sh.n; i += kThreads << wide)
-        each_from(sh, vec(i), i, bound, thr, [&](Key e) {
-          const uint32_t p = atomicAdd(&ts.count, 1u);
-          if (p < kCand) ts.cand[p] = e;
-        });
+  const uint32_t hots = ts.hots;
+  if (hots <= kHot) {
+    // a run by as many lanes as it has vectors (a power of two, 32 at most)
+    const uint32_t wide = len > 16 ? 5u : len > 8 ? 4u : len > 4 ? 3u : len > 2 ? 2u : len > 1 ? 1u : 0u;
+#pragma unroll 2
+    for (uint32_t h = threadIdx.x >> wide; h < hots; h += kThreads >> wide) {
+      const uint32_t first = ts.hot[h] >> 8, t = ts.hot[h] & 0xffu;
+      for (uint32_t l = lane & ((1u << wide) - 1); l < len; l += 1u << wide) {
+        const uint32_t i = t + (first * len + l) * kThreads;
+        if (i < sh.n)
+          each_from(sh, vec(sh, i), i, bound, thr, [&](Key e) {
+            const uint32_t p = atomicAdd(&ts.count, 1u);
+            if (p < kCand) ts.cand[p] = e;
+          });
+      }
+    }
   }
   __syncthreads();
   uint32_t found = ts.count;
-  if (found > kCand) {
-    // Many equal values, or great ones that share few threads: bisect the (unique) keys of all elements until
-    // exactly k are left.
-    Key lo = static_cast<Key>(bound) << 32, hi = ~0ull;
-    while (lo < hi) {
-      const Key mid = lo + (hi - lo) / 2 + 1;
-      const uint32_t least = static_cast<uint32_t>(mid >> 32);
-      uint32_t mine = 0;
-      for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-        each_from(sh, vec(i), i, least, key_value(mid), [&](Key e) { mine += e >= mid; });
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      __syncthreads();
-      if (threadIdx.x == 0) ts.count = 0;
-      __syncthreads();
-      if (lane == 0 && mine) atomicAdd(&ts.count, mine);
-      __syncthreads();
-      const uint32_t at = ts.count;
-      if (at >= k) lo = mid;
-      else hi = mid - 1;
-      if (at == k) break;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) ts.count = 0;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < sh.n; i += kThreads)
-      each_from(sh, vec(i), i, static_cast<uint32_t>(lo >> 32), key_value(lo), [&](Key e) {
-        if (e >= lo) ts.cand[atomicAdd(&ts.count, 1u)] = e;
-      });
-    __syncthreads();
-    found = ts.count;
-  }
+  if (found > kCand || hots > kHot) found = top_overflow(sh.x, sh.V, blocks, rank, vec, bound, k, ts);
   for (uint32_t i = threadIdx.x; i < found; i += kThreads) {
     const Key e = ts.cand[i];
     uint32_t ahead = 0;
@@ -602,23 +687,38 @@ __device__ __forceinline__ uint32_t count_above(const Key* list, uint32_t n, Key
   return lo;
 }
 
+// The given token, kept by one thread of the last warp: the first has the selection to prepare.
+struct Label {
+  int32_t id;
+  float x;
+};
+template <class T>
+__device__ __forceinline__ Label load_label(const seeml_b200_token_scores& d, size_t r, const Share<T>& sh) {
+  Label lab{-1, 0.0f};
+  if (threadIdx.x == kThreads - 1 && d.logprob) {
+    lab.id = d.labels[r];
+    if (lab.id >= 0) lab.x = static_cast<uint32_t>(lab.id) < sh.V ? Ty<T>::to(sh.x[lab.id]) : nan_f();
+  }
+  return lab;
+}
 // The results of a row from its statistics and its blocks' lists of alternatives.
-__device__ __forceinline__ void write_scores(const seeml_b200_token_scores& d, size_t r, const Stats& row, int32_t lab, float xl,
+__device__ __forceinline__ void write_scores(const seeml_b200_token_scores& d, size_t r, const Stats& row, Label lab,
                                              const Key* lists, uint32_t blocks) {
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
-  if (threadIdx.x >= blocks * K && threadIdx.x >= 32) return;
+  if (threadIdx.x >= blocks * K && threadIdx.x >= 32 && threadIdx.x < kThreads - 32) return;
   const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
   auto logprob = [&](float x) {
     return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
   };
   if (threadIdx.x == 0) {
-    if (d.logprob) d.logprob[r] = lab < 0 ? 0.0f : static_cast<uint32_t>(lab) >= V ? nan_f() : logprob(xl);
     if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
     if (d.stats) {
       d.stats[2 * r] = row.m;
       d.stats[2 * r + 1] = row.s;
     }
   }
+  if (threadIdx.x == kThreads - 1 && d.logprob)
+    d.logprob[r] = lab.id < 0 ? 0.0f : static_cast<uint32_t>(lab.id) >= V ? nan_f() : logprob(lab.x);
   for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
     const Key e = lists[i];
     if (e == 0) continue;                              // fewer than K of the block's elements reach the bound
@@ -651,13 +751,8 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   sh.load(sm);
   if (blocks > 1) cluster_arrive(false);               // waited for ahead of the first write to another block
   if (threadIdx.x == 0) ts.hots = ts.count = 0;
-  // the given token's logit comes from memory: it may lie in any block's share
-  int32_t lab = -1;
-  float xl = 0.0f;
-  if (rank == 0 && threadIdx.x == 0 && d.logprob) {
-    lab = d.labels[r];
-    if (lab >= 0) xl = static_cast<uint32_t>(lab) < V ? Ty<T>::to(sh.x[lab]) : nan_f();
-  }
+  Label lab{-1, 0.0f};
+  if (rank == 0) lab = load_label(d, r, sh);           // from memory: it may lie in any block's share
   const float c = kLog2e / d.temperature;
   sh.wait();                                           // every thread reads only what it copied itself
   const float tmax = thread_max<T>(sm, sh.n);
@@ -684,7 +779,8 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   if (K) {
     uint32_t bound = ts.bound[0];
     for (uint32_t b = 1; b < blocks; ++b) bound = min(bound, ts.bound[b]);
-    block_top(sh, [&](uint32_t i) { return sm[i]; }, key, bound, K, ts, (blocks == 1 ? lists : cl.map_shared_rank(lists, 0)) + rank * K);
+    block_top(sh, blocks, rank, ParkedVecs{sm}, key, bound, K, ts, (blocks == 1 ? lists : cl.map_shared_rank(lists, 0)) + rank * K,
+              nullptr, 1, (sh.n + kThreads - 1) / kThreads);
   }
   if (blocks > 1) {
     cluster_arrive(first_warp || K != 0);
@@ -693,7 +789,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   } else {
     __syncthreads();
   }
-  write_scores(d, r, row_stats(ss, c, blocks), lab, xl, lists, blocks);
+  write_scores(d, r, row_stats(ss, c, blocks), lab, lists, blocks);
 }
 
 // The same of a row that one block streams; the selection reads the few vectors it needs a second time (from L2).
@@ -702,20 +798,17 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   __shared__ StatsShared ss;
   __shared__ TopShared ts;
   __shared__ Key list[kTopMax];
+  __shared__ float runs[kSegs * kThreads];
   cg::cluster_group cl = cg::this_cluster();
   const size_t r = blockIdx.x;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
   const bool first_warp = threadIdx.x < 32;
   const Share<T> sh(d.logits, r, d.row_stride, V, 1, 0);
   if (threadIdx.x == 0) ts.hots = ts.count = 0;
-  int32_t lab = -1;
-  float xl = 0.0f;
-  if (threadIdx.x == 0 && d.logprob) {
-    lab = d.labels[r];
-    if (lab >= 0) xl = static_cast<uint32_t>(lab) < V ? Ty<T>::to(sh.x[lab]) : nan_f();
-  }
   const float c = kLog2e / d.temperature;
-  const Stats a = stream_stats<T, ENT>(sh, c, nullptr);
+  const uint32_t batches = (sh.n + kBatchVecs - 1) / kBatchVecs, per_run = (batches + kSegs - 1) / kSegs;
+  const Stats a = stream_stats<T, ENT>(sh, c, nullptr, K ? runs : nullptr, per_run);
+  const Label lab = load_label(d, r, sh);
   const float wmax = warp_max_nan(a.m);
   if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
   const uint32_t key = threadIdx.x < sh.n ? order_key(a.m) : 0u;
@@ -729,9 +822,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   }
   __syncthreads();
   if (first_warp) send_block_stats(ss, m, cl, 0, 1, 1);
-  if (K) block_top(sh, [&](uint32_t i) { return row_vec(sh, i); }, key, ts.bound[0], K, ts, list);
+  if (K) block_top(sh, 1, 0, RowVecs(), key, ts.bound[0], K, ts, list, runs,
+                   (batches + per_run - 1) / per_run, per_run * kBatch);
   __syncthreads();
-  write_scores(d, r, ss.block[0], lab, xl, list, 1);
+  write_scores(d, r, ss.block[0], lab, list, 1);
 }
 
 // ---- gradient of the scores ----------------------------------------------------------------------
@@ -1165,7 +1259,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_stream_kernel(DistillArgs
   if (entries) entries_exp(V, K, tail, a.inv_t, base, th, e);
   __syncthreads();
   const float c = kLog2e / d.temperature;
-  const Stats mine = stream_stats<T, false>(sh, c, named);
+  const Stats mine = stream_stats<T, false>(sh, c, named, nullptr, 0);
   const float wmax = warp_max_nan(mine.m);
   if ((threadIdx.x & 31) == 0) ss.m[threadIdx.x >> 5] = wmax;
   __syncthreads();
