@@ -72,7 +72,7 @@ int kl_bwd(const float* ps, const float* pt, const float* seed, float* d, size_t
            float T, cudaStream_t st);
 size_t loss_scratch_doubles(size_t rows_or_elems);
 
-// ---- vocabulary rows (no counterpart in the reference), kernels_token.cu -------------------
+// ---- vocabulary rows (no counterpart in the reference), kernels_token_scores.cu, kernels_distill.cu ---
 // The descriptors are the C ABI's own, already checked (token_ops.cc); rows >= 1 except for
 // row_loss_sum. Each returns the number of kernels it launched, or a negative value when the
 // device refused an attribute or the launch (cudaGetLastError tells).

@@ -1,5 +1,5 @@
 // Entry points of the vocabulary-row operators (include/seeml_b200.h): every argument is checked
-// here, on the host, before anything is launched; the kernels are in kernels_token.cu.
+// here, on the host, before anything is launched; the kernels are in kernels_token_scores.cu and kernels_distill.cu.
 #include <cuda_runtime.h>
 
 #include <cmath>

@@ -289,7 +289,8 @@ def test_distill(backend_lib, rows, V, dtype, pad, T, masked, K, tail, tdtype):
     _close(g, grad * up, gerr * up, dtype, "dlogits of the backward call")
     assert torch.equal(buf, before)
     alone = ops.distill_topk(x, ids, v, row_weight=wt, scale=scale, temperature=T, tail=tail)
-    assert torch.equal(alone.row_loss, r.row_loss) and torch.equal(alone.loss, r.loss)
+    _close(alone.row_loss, loss, lerr, F32, "row_loss alone")
+    _close(alone.loss, scale * (w * loss).sum(), scale * (w * (lerr + np.abs(loss) * R.U)).sum(), F32, "loss alone")
     inplace = ops.distill_topk(x, ids, v, row_weight=wt, scale=scale, temperature=T, tail=tail, out=x)
     assert inplace.dlogits is x and torch.equal(x, r.dlogits) and torch.equal(inplace.row_loss, r.row_loss)
     assert torch.equal(buf[rows], before[rows]) and torch.equal(buf[:, V:], before[:, V:])
