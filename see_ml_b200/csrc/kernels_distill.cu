@@ -15,215 +15,242 @@ namespace seeml_b200 {
 namespace k {
 namespace {
 
-constexpr int kEntryWarps = kTopMax / 32;
-
-// The teacher's side of one row: thread i < top_k holds entry i, warps without entries skip it. It
-// is worked out in 64 bits while the row is on its way: a loss near 0 is a difference of much
-// larger terms.
-struct Entry {
-  int32_t id;          // -1: absent (or beyond the list)
-  bool first;          // no earlier entry names the token
-  float v, x;          // the teacher's value, the student's logit
-  double q, e;         // exp(value - the greatest, or 0 with a tail); exp((x - the warp's greatest) / T) of a first entry
+// A block has NT threads that work on its share of the row and one more warp for what there is once
+// per row: the teacher's entries while the row is on its way, the factors of the gradient between
+// its two sweeps, the loss during the second. (With that work in the first of the row's own warps a
+// block of 16384 x 32000 f32 in clusters of four lived 22.0 k cycles, 8.4 k of them for it.)
+constexpr int kPer = kTopMax / 32;       // entries of a lane: lane, lane + 32, ...
+struct Entries {
+  int32_t id[kPer];                      // -1: absent (or beyond the list)
+  double q[kPer];                        // exp(value - the greatest, or 0 with a tail)
+  float e[kPer];                         // exp((x - base) / T) of the entry that names its token first
+  uint32_t first;                        // those entries, a bit each
+  float base;                            // the greatest logit of a named token
+  double z, s, l;                        // sums of q, of e, of q (value - greatest - (x - base) / T)
+  double qsum, rest, inv_z;              // the teacher's mass on named and unnamed tokens; q to probability
+  bool bad, dup;                         // a token beyond the vocabulary; one named twice
 };
 struct TeacherShared {
   __align__(16) int32_t id[kTopMax];
   double q[kTopMax];
-  // of the warps with entries: sums of Entry::q, of Entry::e, of q (value - greatest - (x - x greatest) / T)
-  double z[kEntryWarps], s[kEntryWarps], l[kEntryWarps];
-  float v[kEntryWarps], x[kEntryWarps];      // greatest value and logit
-  // of the gradient, once the row is known: unnamed tokens get A exp((x - mt) / T), named ones Entry::e times their
-  // warp's factor less Entry::q inv_z, times the upstream gradient
-  float A, mt, named[kEntryWarps];
-  double inv_z;
-  int bad, dup, empty; // a token beyond the vocabulary; one named twice; no unmasked token in the student's row
+  float A, mt;                           // unnamed tokens' gradient: A exp((x - mt) / T)
 };
-__device__ __forceinline__ bool entry_warp(uint32_t K) { return (threadIdx.x & ~31u) < K; }
-__device__ __forceinline__ float entry_max(const float* part, uint32_t K) {
-  float m = part[0];
-  for (uint32_t w = 1; 32 * w < K; ++w) m = max_nan(m, part[w]);
-  return m;
-}
-__device__ __forceinline__ Entry load_entry(const seeml_b200_distill_topk& d, size_t r) {
-  Entry e{-1, false, -INFINITY, -INFINITY, 0.0, 0.0};
-  if (threadIdx.x < d.top_k) {
-    e.id = d.teacher_id[r * d.top_k + threadIdx.x];
-    const float v = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * d.top_k + threadIdx.x);
-    if (e.id >= 0) e.v = v;
-  }
-  return e;
-}
-// A barrier has to follow.
-__device__ __forceinline__ void publish_entries(uint32_t K, TeacherShared& th, const Entry& e) {
-  if (threadIdx.x == 0) th.bad = th.dup = 0;
-  if (!entry_warp(K)) return;
-  th.id[threadIdx.x] = e.id;
-  const float vm = warp_max_nan(e.v);
-  if ((threadIdx.x & 31) == 0) th.v[threadIdx.x >> 5] = vm;
-}
-// Warps with entries, behind that barrier and ahead of another: the exponentials of both sides, which entries are the
-// first to name their token, and the sums over the warp.
-__device__ __forceinline__ void entries_exp(uint32_t V, uint32_t K, bool tail, double inv_t, TeacherShared& sh, Entry& e) {
-  const uint32_t i = threadIdx.x, w = i >> 5;
-  float shift = tail ? 0.0f : entry_max(sh.v, K);
-  if (shift == -INFINITY) shift = 0.0f;
-  if (e.id >= 0) {
-    if (static_cast<uint32_t>(e.id) >= V) sh.bad = 1;
-    uint32_t same = 0;                       // entries before this one that name its token
-    const int4* id4 = reinterpret_cast<const int4*>(sh.id);
-#pragma unroll 4
-    for (uint32_t j = 0; 4 * j < i; ++j) {
-      const int4 o = id4[j];
-      same += (o.x == e.id && 4 * j < i) + (o.y == e.id && 4 * j + 1 < i) + (o.z == e.id && 4 * j + 2 < i) +
-              (o.w == e.id && 4 * j + 3 < i);
-    }
-    e.first = same == 0;
-    if (same) sh.dup = 1;
-    e.q = exp(static_cast<double>(e.v) - shift);
-  }
-  const float base = warp_max_nan(e.x);
-  const double y = (static_cast<double>(e.x) - base) * inv_t;
-  if (e.first && e.x != -INFINITY) e.e = exp(y);
-  double l = 0.0;
-  if (e.q != 0.0) l = e.x == -INFINITY ? INFINITY : e.q * (static_cast<double>(e.v) - shift - y);
-  sh.q[i] = e.q;
-  const double z = warp_sum(e.q), s = warp_sum(e.e);
-  l = warp_sum(l);
-  if ((i & 31) == 0) { sh.z[w] = z; sh.s[w] = s; sh.l[w] = l; sh.x[w] = base; }
-}
-// What a row's sums become: the entries' sum, the teacher's named and unnamed mass, the student's maximum and sum.
-struct RowSums {
-  double z, qsum, rest;
-  float m, S;
-};
-// exp(d / T) for d <= 0, with the rounding of the exponent made good.
-__device__ __forceinline__ float exp_of(float d, double log2e_t) {
-  const double y = d * log2e_t;
-  const float hi = static_cast<float>(y);
-  const float e = ex2(hi);
-  return e == 0.0f ? 0.0f : fmaf(e, static_cast<float>(y - hi) * static_cast<float>(kLn2), e);
-}
-__device__ __forceinline__ RowSums teacher_sums(const TeacherShared& th, uint32_t K, bool tail) {
-  RowSums r;
-  r.z = th.z[0];
-  for (uint32_t w = 1; 32 * w < K; ++w) r.z += th.z[w];
-  r.qsum = tail ? r.z : r.z == 0.0 ? 0.0 : r.z != r.z ? r.z : 1.0;
-  r.rest = tail && r.qsum < 1.0 ? 1.0 - r.qsum : 0.0;
-  return r;
-}
-// The student's sum over all tokens at the row's maximum, from that over the unnamed ones.
-__device__ __forceinline__ void student_sum(RowSums& r, const TeacherShared& th, uint32_t K, const Stats& row, double log2e_t) {
-  r.m = max_nan(row.m, entry_max(th.x, K));
-  r.S = row.s != 0.0f ? row.s * exp_of(row.m - r.m, log2e_t) : 0.0f;
-  for (uint32_t w = 0; 32 * w < K; ++w) {
-    const float s = static_cast<float>(th.s[w]);
-    if (s != 0.0f) r.S += s * exp_of(th.x[w] - r.m, log2e_t);
-  }
-  if (r.m != r.m) r.S = nan_f();
-}
-// Factors of the gradient; mt and st are the maximum and sum over the unnamed tokens.
-__device__ __forceinline__ void distill_factors(TeacherShared& th, uint32_t K, bool tail, float up_t, float mt, float st,
-                                                const RowSums& r, double log2e_t) {
-  const float rest = st == 0.0f ? 0.0f : static_cast<float>(r.rest), Q = static_cast<float>(r.qsum) + rest;
-  const float inv_s = 1.0f / r.S;
-  float A = 0.0f;
-  if (st != 0.0f && r.S != 0.0f) A = up_t * (Q * exp_of(mt - r.m, log2e_t) * inv_s - rest / st);
-  if (th.bad || r.S != r.S) A = nan_f();
-  th.A = A;
-  th.mt = mt == -INFINITY ? 0.0f : mt;
-  th.empty = r.S == 0.0f;
-  th.inv_z = tail ? 1.0 : r.z == 0.0 ? 0.0 : 1.0 / r.z;
-  for (uint32_t w = 0; 32 * w < K; ++w)
-    th.named[w] = r.S != r.S ? r.S : r.S == 0.0f || th.x[w] == -INFINITY ? 0.0f : Q * exp_of(th.x[w] - r.m, log2e_t) * inv_s;
-}
-// A named token's gradient, over what the sweep of its block left there (behind a barrier).
-template <class T>
-__device__ __forceinline__ void store_named(T* g, uint32_t K, const TeacherShared& th, const Entry& e, float up_t) {
-  double q = e.q;
-  if (th.dup) {
-    q = 0.0;
-    for (uint32_t j = 0; j < K; ++j)
-      if (th.id[j] == e.id) q += th.q[j];
-  }
-  g[e.id] = Ty<T>::from(
-      th.empty ? 0.0f : static_cast<float>(static_cast<double>(up_t) * (e.e * th.named[threadIdx.x >> 5] - q * th.inv_z)));
-}
-
-enum Mode { kLoss, kStep, kBackward };
 struct DistillArgs {
   seeml_b200_distill_topk d;
-  const float* saved_in;       // kBackward
-  const float* upstream;       // kBackward: d loss / d row_loss
-  double inv_t, log2e_t;       // 1 / T, log2(e) / T
+  const float* saved_in;                 // backward call
+  const float* upstream;                 // backward call: d loss / d row_loss
+  double inv_t;                          // 1 / T
+  float c_hi, c_lo;                      // log2(e) / T in two terms
 };
 
-// The loss of a row, and what a backward call needs: one thread, behind the gradient that nobody waits for.
-__device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, const TeacherShared& th, const Stats& row) {
-  const seeml_b200_distill_topk& d = a.d;
-  const uint32_t K = d.top_k;
-  const bool tail = d.tail != 0;
-  RowSums t = teacher_sums(th, K, tail);
-  student_sum(t, th, K, row, a.log2e_t);
-  const double log_s = ln_sum(t.S), inv_z = tail ? 1.0 : t.z == 0.0 ? 0.0 : 1.0 / t.z;
-  double l = 0.0;
-  if (t.S == 0.0f) {                         // nothing left of the student's row
-    if (t.qsum != 0.0) l = INFINITY;
-  } else {
-    for (uint32_t w = 0; 32 * w < K; ++w)
-      if (th.z[w] != 0.0) l += (th.l[w] + th.z[w] * ((static_cast<double>(t.m) - th.x[w]) * a.inv_t)) * inv_z;
-    if (t.qsum != 0.0) l += t.qsum * (log_s - (tail ? 0.0 : ln_sum(static_cast<float>(t.z))));
-    if (t.rest > 0.0 && row.s != 0.0f)
-      l += t.rest * (log(t.rest) - ((static_cast<double>(row.m) - t.m) * a.inv_t + ln_sum(row.s) - log_s));
+__device__ __forceinline__ float4 load4(const float* p) { return make_float4(p[0], p[1], p[2], p[3]); }
+// exp(d / T) for d <= 0, with the rounding of the exponent made good.
+__device__ __forceinline__ float exp_of(float d, const DistillArgs& a) {
+  const float hi = d * a.c_hi, e = ex2(hi);
+  return e == 0.0f ? 0.0f : fmaf(e, (fmaf(d, a.c_hi, -hi) + d * a.c_lo) * static_cast<float>(kLn2), e);
+}
+// The entry warp: its entries' tokens and values.
+__device__ __forceinline__ void load_entries(const seeml_b200_distill_topk& d, size_t r, Entries& e, float (&v)[kPer]) {
+  const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+  for (int w = 0; w < kPer; ++w) {
+    const uint32_t i = lane + 32 * w;
+    e.id[w] = -1;
+    v[w] = -INFINITY;
+    if (i < d.top_k) {
+      e.id[w] = d.teacher_id[r * d.top_k + i];
+      const float value = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * d.top_k + i);
+      if (e.id[w] >= 0) v[w] = value;
+    }
   }
-  d.row_loss[r] = th.bad ? nan_f() : static_cast<float>(l);
+}
+// The teacher's mass from the sum of its exponentials.
+__device__ __forceinline__ void entries_mass(Entries& e, bool tail) {
+  e.qsum = tail ? e.z : e.z == 0.0 ? 0.0 : e.z != e.z ? e.z : 1.0;
+  e.rest = tail && e.qsum < 1.0 ? 1.0 - e.qsum : 0.0;
+  e.inv_z = tail ? 1.0 : e.z == 0.0 ? 0.0 : 1.0 / e.z;
+}
+// exp(y) to a little over an ulp of f32, whatever the magnitude of y.
+__device__ __forceinline__ float exp_near(double y) {
+  const float hi = static_cast<float>(y), e = expf(hi);
+  return e == 0.0f ? 0.0f : fmaf(e, static_cast<float>(y - hi), e);
+}
+// The entry warp: both sides' exponentials and their sums, the teacher's in 64 bits (what is left of its mass is a
+// difference from 1, and may meet a logarithm in the hundreds); x: the student's logits of the entries, -inf where they
+// do not count.
+__device__ __forceinline__ void entries_exp(uint32_t V, uint32_t K, bool tail, double inv_t, const float (&v)[kPer],
+                                            const float (&x)[kPer], TeacherShared& sh, Entries& e) {
+  const uint32_t lane = threadIdx.x & 31;
+  float vm = -INFINITY, xm = -INFINITY;
+  bool bad = false;
+#pragma unroll
+  for (int w = 0; w < kPer; ++w) {
+    sh.id[lane + 32 * w] = e.id[w];
+    bad |= e.id[w] >= 0 && static_cast<uint32_t>(e.id[w]) >= V;
+    vm = max_nan(vm, v[w]);
+    xm = max_nan(xm, x[w]);
+  }
+  e.bad = __any_sync(0xffffffffu, bad);
+  vm = warp_max_nan(vm);
+  e.base = warp_max_nan(xm);
+  __syncwarp();
+  // entries that name the same token, the entry itself among them
+  uint32_t same[kPer] = {0, 0, 0, 0};
+  const int4* id4 = reinterpret_cast<const int4*>(sh.id);
+#pragma unroll 4
+  for (uint32_t j = 0; 4 * j < K; ++j) {
+    const int4 o = id4[j];
+#pragma unroll
+    for (int w = 0; w < kPer; ++w)
+      if (32 * w < K) same[w] += (o.x == e.id[w]) + (o.y == e.id[w]) + (o.z == e.id[w]) + (o.w == e.id[w]);
+  }
+  bool dup = false;
+  e.first = 0;
+#pragma unroll
+  for (int w = 0; w < kPer; ++w)
+    if (e.id[w] >= 0) {
+      dup |= same[w] > 1;
+      e.first |= 1u << w;
+    }
+  e.dup = __any_sync(0xffffffffu, dup);
+  if (e.dup) {                           // of those, only the first one counts
+    for (uint32_t j = 0; j < K; ++j)
+#pragma unroll
+      for (int w = 0; w < kPer; ++w)
+        if (sh.id[j] == e.id[w] && j < lane + 32 * w) e.first &= ~(1u << w);
+  }
+  const double shift = tail || vm == -INFINITY ? 0.0 : vm;
+  e.z = e.s = e.l = 0.0;
+#pragma unroll
+  for (int w = 0; w < kPer; ++w) {
+    e.q[w] = 0.0;
+    e.e[w] = 0.0f;
+    if (32 * w >= K) continue;
+    if (e.id[w] >= 0) {
+      const double y = (static_cast<double>(x[w]) - e.base) * inv_t;
+      e.q[w] = exp(static_cast<double>(v[w]) - shift);
+      if ((e.first >> w & 1u) && x[w] != -INFINITY) e.e[w] = exp_near(y);
+      if (e.q[w] != 0.0) e.l += x[w] == -INFINITY ? INFINITY : e.q[w] * (static_cast<double>(v[w]) - shift - y);
+      e.z += e.q[w];
+      e.s += e.e[w];
+    }
+    sh.q[lane + 32 * w] = e.q[w];
+  }
+  e.z = warp_sum(e.z);
+  e.s = warp_sum(e.s);
+  e.l = warp_sum(e.l);
+  entries_mass(e, tail);
+}
+// The student's maximum and sum over all tokens, from those over the unnamed ones.
+__device__ __forceinline__ Stats student_sum(const Entries& e, const Stats& row, const DistillArgs& a) {
+  const float es = static_cast<float>(e.s);
+  Stats r{max_nan(row.m, e.base), 0.0f, 0.0f};
+  if (row.s != 0.0f) r.s = row.s * exp_of(row.m - r.m, a);
+  if (es != 0.0f) r.s += es * exp_of(e.base - r.m, a);
+  if (r.m != r.m) r.s = nan_f();
+  return r;
+}
+// Factors of the gradient: unnamed tokens get A exp((x - mt) / T), Entries::e is multiplied with what is returned
+// (unnamed: the statistics of the unnamed tokens, all: of every token).
+__device__ __forceinline__ float gradient_factors(float& A, float& mt, const Entries& e, float up_t, const Stats& unnamed,
+                                                  const Stats& all, const DistillArgs& a) {
+  const float rest = unnamed.s == 0.0f ? 0.0f : static_cast<float>(e.rest), Q = static_cast<float>(e.qsum) + rest;
+  const float inv_s = 1.0f / all.s;
+  float named = 0.0f;
+  A = 0.0f;
+  if (unnamed.s != 0.0f && all.s != 0.0f) A = up_t * (Q * exp_of(unnamed.m - all.m, a) * inv_s - rest / unnamed.s);
+  if (all.s != 0.0f && e.base != -INFINITY) named = Q * exp_of(e.base - all.m, a) * inv_s;
+  if (all.s != all.s) A = named = all.s;
+  if (e.bad) A = nan_f();
+  mt = unnamed.m == -INFINITY ? 0.0f : unnamed.m;
+  return named;
+}
+// The named tokens' gradient over what the sweep left there (behind a barrier): those with a place in this block's share.
+template <class T, int NT>
+__device__ __forceinline__ void store_named(T* g, const Share<T, NT>& sh, uint32_t K, const TeacherShared& th, const Entries& e,
+                                            float up_t, float named, bool empty) {
+  if (e.bad) return;
+#pragma unroll
+  for (int w = 0; w < kPer; ++w) {
+    if (!((e.first >> w) & 1u) || sh.local(e.id[w]) < 0) continue;
+    double q = e.q[w];
+    if (e.dup) {
+      q = 0.0;
+      for (uint32_t j = 0; j < K; ++j)
+        if (th.id[j] == e.id[w]) q += th.q[j];
+    }
+    g[e.id[w]] = Ty<T>::from(empty ? 0.0f : static_cast<float>(up_t * (static_cast<double>(e.e[w]) * named - q * e.inv_z)));
+  }
+}
+// The loss of a row, and what a backward call needs: one thread.
+__device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, const Entries& e, const Stats& unnamed, const Stats& all) {
+  const seeml_b200_distill_topk& d = a.d;
+  double l = 0.0;
+  if (all.s == 0.0f) {                   // nothing left of the student's row
+    if (e.qsum != 0.0) l = INFINITY;
+  } else {
+    const double log_s = ln_sum(all.s);
+    if (e.qsum != 0.0)
+      l = (e.l + e.z * ((static_cast<double>(all.m) - e.base) * a.inv_t)) * e.inv_z +
+          e.qsum * (log_s - (d.tail ? 0.0 : ln_sum(static_cast<float>(e.z))));
+    if (e.rest > 0.0 && unnamed.s != 0.0f)
+      l += e.rest * (log(e.rest) - ((static_cast<double>(unnamed.m) - all.m) * a.inv_t + ln_sum(unnamed.s) - log_s));
+  }
+  d.row_loss[r] = e.bad ? nan_f() : static_cast<float>(l);
   if (d.saved) {
     float* sv = d.saved + 4 * r;
-    sv[0] = row.m; sv[1] = row.s; sv[2] = t.m; sv[3] = t.S;
+    sv[0] = unnamed.m; sv[1] = unnamed.s; sv[2] = all.m; sv[3] = all.s;
   }
 }
-// A row of weight 0, or this block's share of it.
+__device__ __forceinline__ void skipped_loss(const seeml_b200_distill_topk& d, size_t r) {
+  d.row_loss[r] = 0.0f;
+  if (d.saved) {
+    float* sv = d.saved + 4 * r;
+    sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;
+  }
+}
+// The entry warp: the words of thread_stats that leave the named tokens out, n bytes at 16.
 template <class T, int NT>
-__device__ __forceinline__ void skip_row(const DistillArgs& a, size_t r, const Share<T, NT>& sh, T* g, bool same, bool loss) {
-  const seeml_b200_distill_topk& d = a.d;
-  if (g) {
-    float2 f[Ty<T>::E / 2];
+__device__ __forceinline__ void mark_named(uint32_t* words, uint32_t bytes, const Entries& e, const Share<T, NT>& sh) {
+  for (uint32_t i = threadIdx.x & 31; i < bytes / 16; i += 32) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
+  __syncwarp();
 #pragma unroll
-    for (int q = 0; q < Ty<T>::E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
-    for (uint32_t i = threadIdx.x; i < sh.n; i += NT) {
-      const int j = sh.elem(i);
-      if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + j) = make_uint4(0, 0, 0, 0);
-      else store_elems<T>(g, j, sh.V, f);
-    }
-  }
-  if (loss && threadIdx.x == 0) {
-    d.row_loss[r] = 0.0f;
-    if (d.saved) {
-      float* sv = d.saved + 4 * r;
-      sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;
-    }
+  for (int w = 0; w < kPer; ++w) {
+    const int at = e.id[w] >= 0 && static_cast<uint32_t>(e.id[w]) < sh.V ? sh.local(e.id[w]) : -1;
+    if (at < 0) continue;
+    const uint32_t i = static_cast<uint32_t>(at) / Ty<T>::E;
+    atomicOr(&words[i / (kBatch * NT) * NT + i % NT], 1u << (i % (kBatch * NT) / NT * 8 + static_cast<uint32_t>(at) % Ty<T>::E));
   }
 }
-// The words of thread_stats that leave the named tokens out: zeroed ahead of a barrier, set ahead of another.
+// The entry warp: the student's logits of its entries.
 template <class T, int NT>
-__device__ __forceinline__ void clear_named(const Share<T, NT>& sh, uint32_t* named) {
-  for (uint32_t b = 0; b < sh.batches(); ++b) named[b * NT + threadIdx.x] = 0;
+__device__ __forceinline__ void load_logits(const Share<T, NT>& sh, const Entries& e, float (&x)[kPer]) {
+#pragma unroll
+  for (int w = 0; w < kPer; ++w)
+    x[w] = e.id[w] >= 0 && static_cast<uint32_t>(e.id[w]) < sh.V ? Ty<T>::to(sh.x[e.id[w]]) : -INFINITY;
 }
+// Zeros over this block's share.
 template <class T, int NT>
-__device__ __forceinline__ void set_named(const Share<T, NT>&, uint32_t* named, uint32_t at) {
-  constexpr uint32_t E = Ty<T>::E;
-  const uint32_t i = at / E;
-  atomicOr(&named[i / (kBatch * NT) * NT + i % NT], 1u << (i % (kBatch * NT) / NT * 8 + at % E));
+__device__ __forceinline__ void store_zeros(const Share<T, NT>& sh, T* g, bool same) {
+  float2 f[Ty<T>::E / 2];
+#pragma unroll
+  for (int q = 0; q < Ty<T>::E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
+  for (uint32_t i = threadIdx.x; i < sh.n; i += NT) {
+    if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + sh.elem(i)) = make_uint4(0, 0, 0, 0);
+    else store_elems<T>(g, sh.elem(i), sh.V, f);
+  }
 }
-// The gradient of this block's share but for the named tokens, which the caller writes over it.
+// The gradient of this block's share but for the named tokens.
 template <class T, int NT, class Source>
 __device__ __forceinline__ void sweep(const Share<T, NT>& sh, Source src, T* g, bool same, float A, float mt, float c) {
   constexpr int E = Ty<T>::E;
   const float2 shift = make_float2(-mt, -mt), c2 = make_float2(c, c), A2 = make_float2(A, A);
   const uint32_t batches = sh.batches();
   src.begin(sh);
-  for (uint32_t b = 0; b < batches; ++b) {
+  for (uint32_t o = 0; o < batches; ++o) {
     uint4 v[kBatch];
-    src.batch(sh, b, batches, v);
+    src.batch(sh, o, batches, v);
+    const uint32_t b = Source::kBackwards ? batches - 1 - o : o;
     const uint32_t i = b * Share<T, NT>::kStep + threadIdx.x;
     T* dst = g + sh.elem(i);
     const bool fast = same && sh.whole_batch(b);
@@ -243,9 +270,12 @@ __device__ __forceinline__ void sweep(const Share<T, NT>& sh, Source src, T* g, 
 }
 
 // A row parked in the shared memory of one block, or of a cluster of them.
+// The block's barrier, for warps that meet it at different places of the code.
+template <int Threads>
+__device__ __forceinline__ void meet() { asm volatile("barrier.sync 1, %0;" ::"n"(Threads) : "memory"); }
 constexpr int kParkThreads = 128;
-template <class T, int MODE>
-__global__ void __launch_bounds__(kParkThreads) distill_kernel(DistillArgs a, uint32_t share, uint32_t blocks) {
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(kParkThreads + 32) distill_kernel(DistillArgs a, uint32_t share, uint32_t blocks) {
   constexpr int NT = kParkThreads;
   extern __shared__ uint4 sm[];
   __shared__ TeacherShared th;
@@ -255,79 +285,79 @@ __global__ void __launch_bounds__(kParkThreads) distill_kernel(DistillArgs a, ui
   const uint32_t rank = blockIdx.x % blocks;           // blocks of a row follow each other, as a cluster's do
   const size_t r = blockIdx.x / blocks;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
-  const bool tail = d.tail != 0, first_warp = threadIdx.x < 32;
-  uint32_t* named = reinterpret_cast<uint32_t*>(sm + share);
   const Share<T, NT> sh(d.logits, r, d.row_stride, V, blocks, rank);
-  T* g = MODE != kLoss ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
-  const bool same = MODE != kLoss && (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
-  // the row's weight and its entries arrive together; the row is only asked for if it counts
-  const float w = MODE == kBackward ? a.upstream[r] : d.row_weight ? d.row_weight[r] : 1.0f;
-  Entry e = load_entry(d, r);
-  if (MODE != kBackward) clear_named(sh, named);
-  if (w == 0.0f) {                                     // the whole cluster leaves here
-    skip_row(a, r, sh, g, same, MODE != kBackward && rank == 0);
+  T* g = GRAD ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
+  const float c = kLog2e / d.temperature;
+  uint32_t* words = reinterpret_cast<uint32_t*>(sm + share);
+  // the row is only asked for if it counts; otherwise the whole cluster leaves
+  const float w = d.row_weight ? d.row_weight[r] : 1.0f;
+  if (threadIdx.x < NT) {
+    const bool same = GRAD && sh.same_phase(g);
+    if (w == 0.0f) {
+      if (GRAD) store_zeros(sh, g, same);
+      return;
+    }
+    sh.load(sm);
+    if (blocks > 1) cluster_arrive(false);             // waited for ahead of the first write to another block
+    meet<NT + 32>();                                   // the named tokens are marked
+    const Stats mine = thread_stats<T, NT, false>(sh, Parked{sm}, c, words, nullptr, 0);
+    publish_max(ss, mine.m);
+    meet<NT + 32>();
+    publish_sums<false>(ss, mine, c, block_max(ss));
+    if (blocks > 1) cluster_wait();
+    meet<NT + 32>();
+    if (blocks > 1) cluster_arrive(false);
+    if (!GRAD) return;
+    meet<NT + 32>();                                   // the factors are known
+    if (blocks > 1) cluster_wait();
+    sweep(sh, Parked{sm}, g, same, th.A, th.mt, c);
+    meet<NT + 32>();
     return;
   }
-  sh.load(sm);
-  if (MODE != kBackward && blocks > 1) cluster_arrive(false);  // waited for ahead of the first write to another block
-  const bool there = e.id >= 0 && static_cast<uint32_t>(e.id) < V;
-  const int at = there ? sh.local(e.id) : -1;
-  // Read here, ahead of the cluster's barrier: in place, another block may overwrite it behind that. The backward call
-  // has no such barrier and needs only the entries of its own share.
-  if (MODE == kBackward ? at >= 0 : there) e.x = Ty<T>::to(sh.x[e.id]);
-  publish_entries(K, th, e);
-  __syncthreads();
-  if (MODE != kBackward) {
-    if (at >= 0) set_named(sh, named, at);
-    __syncthreads();
+  // the entry warp
+  Entries e;
+  float v[kPer], x[kPer];
+  load_entries(d, r, e, v);
+  if (w == 0.0f) {
+    if (rank == 0 && threadIdx.x == NT) skipped_loss(d, r);
+    return;
   }
-  if (entry_warp(K)) entries_exp(V, K, tail, a.inv_t, th, e);
-  const float c = kLog2e / d.temperature, up_t = (MODE == kBackward ? 1.0f : d.scale) * w / d.temperature;
-  if (MODE != kBackward) {
-    const Stats mine = thread_stats<T, NT, false>(sh, Parked{sm}, c, named, nullptr, 0);
-    publish_max(ss, mine.m);
-    __syncthreads();
-    const float bm = block_max(ss);
-    publish_sums<false>(ss, mine, c, bm);
-    __syncthreads();
-    if (blocks > 1) cluster_wait();
-    if (first_warp) send_block_stats(ss, bm, cl, rank, blocks, MODE == kLoss ? 1 : blocks);
-    if (blocks > 1) {
-      cluster_arrive(first_warp);
-      if (MODE == kLoss && rank != 0) return;
-      cluster_wait();
-    }
-    if (MODE == kStep && threadIdx.x == 0) {
-      const Stats row = row_stats(ss, c, blocks);
-      RowSums t = teacher_sums(th, K, tail);
-      student_sum(t, th, K, row, a.log2e_t);
-      distill_factors(th, K, tail, up_t, row.m, row.s, t, a.log2e_t);
-    }
+  if (blocks > 1) cluster_arrive(false);
+  // read ahead of the cluster's barrier: in place, another block may overwrite it behind that
+  load_logits(sh, e, x);
+  mark_named<T, NT>(words, sh.batches() * NT * 4, e, sh);
+  meet<NT + 32>();
+  entries_exp(V, K, d.tail != 0, a.inv_t, v, x, th, e);
+  meet<NT + 32>();
+  if (blocks > 1) cluster_wait();
+  meet<NT + 32>();
+  send_block_stats(ss, block_max(ss), cl, rank, blocks, GRAD ? blocks : 1);
+  if (blocks > 1) {
+    cluster_arrive(true);
+    if (!GRAD && rank != 0) return;
+    cluster_wait();
   } else {
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      const float* sv = a.saved_in + 4 * r;
-      RowSums t = teacher_sums(th, K, tail);
-      t.m = sv[2];
-      t.S = sv[3];
-      distill_factors(th, K, tail, up_t, sv[0], sv[1], t, a.log2e_t);
-    }
+    __syncwarp();
   }
-  if (MODE != kLoss) {
-    __syncthreads();
-    sweep(sh, Parked{sm}, g, same, th.A, th.mt, c);
-    __syncthreads();
-    if (at >= 0 && e.first && !th.bad) store_named(g, K, th, e, up_t);
+  const Stats unnamed = row_stats(ss, c, blocks), all = student_sum(e, unnamed, a);
+  const float up_t = d.scale * w / d.temperature;
+  float named = 0.0f;
+  if (GRAD) {
+    named = gradient_factors(th.A, th.mt, e, up_t, unnamed, all, a);
+    meet<NT + 32>();
   }
-  if (MODE != kBackward && rank == 0 && threadIdx.x == 0) distill_loss(a, r, th, row_stats(ss, c, blocks));
+  if (rank == 0 && threadIdx.x == NT) distill_loss(a, r, e, unnamed, all);
+  if (GRAD) {
+    meet<NT + 32>();
+    store_named(g, sh, K, th, e, up_t, named, all.s == 0.0f);
+  }
 }
 
-// The loss of a row that one block streams.
-constexpr int kStreamThreads = 256;
-template <class T>
-__global__ void __launch_bounds__(kStreamThreads, 4) distill_stream_kernel(DistillArgs a) {
-  constexpr int NT = kStreamThreads;
-  extern __shared__ uint32_t named[];
+// A row that one block streams: once for the loss, twice for the gradient, the second time from its end, which L2 still
+// holds when it no longer holds the start.
+template <class T, int NT, int MIN_BLOCKS, bool GRAD>
+__global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(DistillArgs a) {
+  extern __shared__ uint32_t words[];
   __shared__ TeacherShared th;
   __shared__ StatsShared<NT> ss;
   const seeml_b200_distill_topk& d = a.d;
@@ -335,29 +365,140 @@ __global__ void __launch_bounds__(kStreamThreads, 4) distill_stream_kernel(Disti
   const size_t r = blockIdx.x;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
   const Share<T, NT> sh(d.logits, r, d.row_stride, V, 1, 0);
+  T* g = GRAD ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
+  const float c = kLog2e / d.temperature;
   const float w = d.row_weight ? d.row_weight[r] : 1.0f;
-  Entry e = load_entry(d, r);
-  clear_named(sh, named);
-  if (w == 0.0f) {
-    skip_row<T, NT>(a, r, sh, nullptr, false, true);
+  if (threadIdx.x < NT) {
+    const bool same = GRAD && sh.same_phase(g);
+    if (w == 0.0f) {
+      if (GRAD) store_zeros(sh, g, same);
+      return;
+    }
+    meet<NT + 32>();                                   // the named tokens are marked
+    const Stats mine = thread_stats<T, NT, false>(sh, Streamed(), c, words, nullptr, 0);
+    publish_max(ss, mine.m);
+    meet<NT + 32>();
+    publish_sums<false>(ss, mine, c, block_max(ss));
+    meet<NT + 32>();
+    if (!GRAD) return;
+    meet<NT + 32>();                                   // the factors are known
+    sweep(sh, StreamedBackwards(), g, same, th.A, th.mt, c);
+    meet<NT + 32>();
     return;
   }
-  const bool there = e.id >= 0 && static_cast<uint32_t>(e.id) < V;
-  if (there) e.x = Ty<T>::to(sh.x[e.id]);
-  publish_entries(K, th, e);
+  Entries e;
+  float v[kPer], x[kPer];
+  load_entries(d, r, e, v);
+  if (w == 0.0f) {
+    if (threadIdx.x == NT) skipped_loss(d, r);
+    return;
+  }
+  load_logits(sh, e, x);
+  mark_named<T, NT>(words, sh.batches() * NT * 4, e, sh);
+  meet<NT + 32>();
+  entries_exp(V, K, d.tail != 0, a.inv_t, v, x, th, e);
+  meet<NT + 32>();
+  meet<NT + 32>();
+  send_block_stats(ss, block_max(ss), cl, 0, 1, 1);
+  __syncwarp();
+  const Stats unnamed = ss.block[0], all = student_sum(e, unnamed, a);
+  const float up_t = d.scale * w / d.temperature;
+  float named = 0.0f;
+  if (GRAD) {
+    named = gradient_factors(th.A, th.mt, e, up_t, unnamed, all, a);
+    meet<NT + 32>();
+  }
+  if (threadIdx.x == NT) distill_loss(a, r, e, unnamed, all);
+  if (GRAD) {
+    meet<NT + 32>();
+    store_named(g, sh, K, th, e, up_t, named, all.s == 0.0f);
+  }
+}
+
+// The gradient alone: the row's sums are given, so its blocks know nothing of each other. Thread i holds entry i.
+constexpr int kGradThreads = 128;
+static_assert(kGradThreads >= kTopMax, "a thread per entry");
+template <class T>
+__global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs a, uint32_t blocks) {
+  constexpr int NT = kGradThreads;
+  extern __shared__ uint4 sm[];
+  __shared__ TeacherShared th;
+  __shared__ float vmax[NT / 32];
+  __shared__ double zsum[NT / 32];
+  const seeml_b200_distill_topk& d = a.d;
+  const uint32_t rank = blockIdx.x % blocks;
+  const size_t r = blockIdx.x / blocks;
+  const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
+  const bool tail = d.tail != 0;
+  const Share<T, NT> sh(d.logits, r, d.row_stride, V, blocks, rank);
+  T* g = static_cast<T*>(d.dlogits) + r * d.grad_stride;
+  const bool same = sh.same_phase(g);
+  const float up = a.upstream[r];
+  const float4 sv = load4(a.saved_in + 4 * r);
+  int32_t id = -1;
+  float v = -INFINITY;
+  if (threadIdx.x < K) {
+    id = d.teacher_id[r * K + threadIdx.x];
+    const float value = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * K + threadIdx.x);
+    if (id >= 0) v = value;
+  }
+  if (up == 0.0f) {
+    store_zeros(sh, g, same);
+    return;
+  }
+  sh.load(sm);
+  const int at = id >= 0 && static_cast<uint32_t>(id) < V ? sh.local(id) : -1;
+  const float x = at >= 0 ? Ty<T>::to(sh.x[id]) : -INFINITY;     // only this block overwrites it
+  th.id[threadIdx.x] = id;
+  const float wm = warp_max_nan(v);
+  if ((threadIdx.x & 31) == 0) vmax[threadIdx.x >> 5] = wm;
+  const bool bad = __syncthreads_or(id >= 0 && static_cast<uint32_t>(id) >= V) != 0;
+  double q = 0.0;
+  if ((threadIdx.x & ~31u) < K) {
+    float vm = vmax[0];
+#pragma unroll
+    for (int w = 1; w < NT / 32; ++w) vm = max_nan(vm, vmax[w]);
+    if (id >= 0) q = exp(static_cast<double>(v) - (tail || vm == -INFINITY ? 0.0f : vm));
+  }
+  th.q[threadIdx.x] = q;
+  uint32_t same_id = 0;
+  if (at >= 0) {
+    const int4* id4 = reinterpret_cast<const int4*>(th.id);
+#pragma unroll 4
+    for (uint32_t j = 0; 4 * j < K; ++j) {
+      const int4 o = id4[j];
+      same_id += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+    }
+  }
+  const double z = warp_sum(q);
+  if ((threadIdx.x & 31) == 0) zsum[threadIdx.x >> 5] = z;
   __syncthreads();
-  if (there) set_named(sh, named, static_cast<uint32_t>(e.id) + sh.phase);
+  Entries e;                                           // what the factors want of it, in every thread
+  e.z = 0.0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) e.z += zsum[w];
+  e.bad = bad;
+  e.base = sv.z;
+  entries_mass(e, tail);
+  const float up_t = up / d.temperature;
+  const Stats unnamed{sv.x, sv.y, 0.0f}, all{sv.z, sv.w, 0.0f};
+  float A, mt;
+  const float named = gradient_factors(A, mt, e, up_t, unnamed, all, a);
+  sweep(sh, Parked{sm}, g, same, A, mt, kLog2e / d.temperature);
+  bool first = true;
+  if (same_id > 1) {                                   // a token named twice: its first entry stands for all
+    q = 0.0;
+    for (uint32_t j = 0; j < K; ++j)
+      if (th.id[j] == id) {
+        q += th.q[j];
+        first = first && j >= threadIdx.x;
+      }
+  }
   __syncthreads();
-  if (entry_warp(K)) entries_exp(V, K, d.tail != 0, a.inv_t, th, e);     // while the other warps stream
-  const float c = kLog2e / d.temperature;
-  const Stats mine = thread_stats<T, NT, false>(sh, Streamed(), c, named, nullptr, 0);
-  publish_max(ss, mine.m);
-  __syncthreads();
-  const float bm = block_max(ss);
-  publish_sums<false>(ss, mine, c, bm);
-  __syncthreads();
-  if (threadIdx.x < 32) send_block_stats(ss, bm, cl, 0, 1, 1);
-  if (threadIdx.x == 0) distill_loss(a, r, th, ss.block[0]);
+  if (at >= 0 && first && !bad) {
+    const float ex = x == -INFINITY ? 0.0f : exp_near((static_cast<double>(x) - sv.z) * a.inv_t);
+    g[id] = Ty<T>::from(all.s == 0.0f ? 0.0f : static_cast<float>(up_t * (static_cast<double>(ex) * named - q * e.inv_z)));
+  }
 }
 
 // loss = scale * sum of weight * row_loss, in a fixed order and 64 bits: one block, four rows in flight per thread.
@@ -382,8 +523,9 @@ __global__ void __launch_bounds__(kSumThreads) row_loss_sum_kernel(const float* 
 }
 
 DistillArgs distill_args(const seeml_b200_distill_topk& d) {
-  const double inv_t = 1.0 / static_cast<double>(d.temperature);
-  return DistillArgs{d, nullptr, nullptr, inv_t, inv_t / kLn2};
+  const double inv_t = 1.0 / static_cast<double>(d.temperature), c = inv_t / kLn2;
+  const float hi = static_cast<float>(c);
+  return DistillArgs{d, nullptr, nullptr, inv_t, hi, static_cast<float>(c - hi)};
 }
 // Bytes of the words that mark the named tokens of a share.
 size_t named_bytes(uint64_t vecs, int threads) { return (vecs + kBatch * threads - 1) / (kBatch * threads) * threads * 4; }
@@ -393,18 +535,18 @@ constexpr uint64_t kMostParked = 34u << 10;
 
 int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
   const DistillArgs a = distill_args(d);
-  const uint64_t elem = elem_bytes(d.dtype);
-  if (!d.dlogits && d.rows >= kManyRows && d.vocab * elem >= (24u << 10))
-    return by_type(d.dtype, [&](auto t) {
-      return launch_rows<distill_stream_kernel<decltype(t)>>(d.rows, 1, false, kStreamThreads,
-                                                             named_bytes(row_vecs(d.vocab, elem), kStreamThreads), st, a);
-    });
-  const Split s = split_row(d.rows, d.vocab, elem, kMostParked);
-  const size_t smem = s.share * 16 + named_bytes(s.share, kParkThreads);
+  const uint64_t elem = elem_bytes(d.dtype), vecs = row_vecs(d.vocab, elem);
+  const bool many = d.rows >= kManyRows;
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
-    return d.dlogits ? launch_rows<distill_kernel<T, kStep>>(d.rows, s.blocks, true, kParkThreads, smem, st, a, s.share, s.blocks)
-                     : launch_rows<distill_kernel<T, kLoss>>(d.rows, s.blocks, true, kParkThreads, smem, st, a, s.share, s.blocks);
+    if (many && !d.dlogits && d.vocab * elem >= (24u << 10))
+      return launch_rows<distill_stream_kernel<T, 256, 3, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a);
+    if (many && d.dlogits && d.vocab * elem > 4 * kMostParked)
+      return launch_rows<distill_stream_kernel<T, 512, 2, true>>(d.rows, 1, false, 512 + 32, named_bytes(vecs, 512), st, a);
+    const Split s = split_row(d.rows, d.vocab, elem, kMostParked);
+    const size_t smem = s.share * 16 + named_bytes(s.share, kParkThreads);
+    return d.dlogits ? launch_rows<distill_kernel<T, true>>(d.rows, s.blocks, true, kParkThreads + 32, smem, st, a, s.share, s.blocks)
+                     : launch_rows<distill_kernel<T, false>>(d.rows, s.blocks, true, kParkThreads + 32, smem, st, a, s.share, s.blocks);
   });
 }
 int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
@@ -427,8 +569,7 @@ int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
   a.saved_in = b.saved;
   a.upstream = b.drow_loss;
   return by_type(b.dtype, [&](auto t) {
-    return launch_rows<distill_kernel<decltype(t), kBackward>>(b.rows, s.blocks, false, kParkThreads, s.share * 16, st, a,
-                                                               s.share, s.blocks);
+    return launch_rows<distill_grad_kernel<decltype(t)>>(b.rows, s.blocks, false, kGradThreads, s.share * 16, st, a, s.blocks);
   });
 }
 int row_loss_sum(const float* row_loss, const float* weight, size_t rows, float scale, float* loss, cudaStream_t st) {

@@ -193,6 +193,10 @@ struct Share {
     return v >= first && v - first < n ? static_cast<int>(static_cast<uint32_t>(j) + phase - first * E) : -1;
   }
   __device__ __forceinline__ uint32_t batches() const { return (n + kStep - 1) / kStep; }
+  // whether a matrix of the same type, row by row, has this row at the same place in its vectors
+  __device__ __forceinline__ bool same_phase(const T* g) const {
+    return (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == phase;
+  }
   // the whole batch b lies inside the row
   __device__ __forceinline__ bool whole_batch(uint32_t b) const { return b * kStep >= lo && (b + 1) * kStep <= hi; }
   // Does f(i) for the (at most two) vectors of this thread that hang over an end.
@@ -273,21 +277,22 @@ __device__ __forceinline__ float block_max(const StatsShared<NT>& sh) {
   for (int w = 1; w < NT / 32; ++w) m = max_nan(m, sh.m[w]);
   return m;
 }
-// First warp only, after a block barrier behind the writes to sh.s and sh.t: this block's statistics, sent to blocks
+// One warp, after a block barrier behind the writes to sh.s and sh.t: this block's statistics, sent to blocks
 // [0, targets) of the cluster (the block alone when it is one). A fixed order: the same bits in every run.
 template <int NT>
 __device__ __forceinline__ void send_block_stats(StatsShared<NT>& sh, float m, cg::cluster_group& cl, uint32_t rank,
                                                  uint32_t blocks, uint32_t targets) {
+  const uint32_t lane = threadIdx.x & 31;
   Stats v;
   v.m = m;
-  v.s = sh.s[threadIdx.x & (NT / 32 - 1)];
-  v.t = sh.t[threadIdx.x & (NT / 32 - 1)];
+  v.s = sh.s[lane & (NT / 32 - 1)];
+  v.t = sh.t[lane & (NT / 32 - 1)];
 #pragma unroll
   for (int o = NT / 64; o > 0; o >>= 1) {
     v.s += __shfl_xor_sync(0xffffffffu, v.s, o);
     v.t += __shfl_xor_sync(0xffffffffu, v.t, o);
   }
-  if (threadIdx.x < targets) (blocks == 1 ? &sh : cl.map_shared_rank(&sh, threadIdx.x))->block[rank] = v;
+  if (lane < targets) (blocks == 1 ? &sh : cl.map_shared_rank(&sh, lane))->block[rank] = v;
 }
 template <int NT>
 __device__ __forceinline__ Stats row_stats(const StatsShared<NT>& sh, float c, uint32_t blocks) {
@@ -347,6 +352,7 @@ __device__ __forceinline__ void row_batch(const Share<T, NT>& sh, uint32_t b, ui
   }
 }
 struct Streamed {
+  static constexpr bool kBackwards = false;
   uint4 next[kBatch];
   template <class T, int NT>
   __device__ __forceinline__ void begin(const Share<T, NT>& sh) { row_batch(sh, 0, next); }
@@ -357,7 +363,20 @@ struct Streamed {
     if (b + 1 < batches) row_batch(sh, b + 1, next);
   }
 };
+struct StreamedBackwards {               // the last batch first
+  static constexpr bool kBackwards = true;
+  uint4 next[kBatch];
+  template <class T, int NT>
+  __device__ __forceinline__ void begin(const Share<T, NT>& sh) { row_batch(sh, sh.batches() - 1, next); }
+  template <class T, int NT>
+  __device__ __forceinline__ void batch(const Share<T, NT>& sh, uint32_t o, uint32_t batches, uint4 (&v)[kBatch]) {
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = next[u];
+    if (o + 1 < batches) row_batch(sh, batches - 2 - o, next);
+  }
+};
 struct Parked {
+  static constexpr bool kBackwards = false;
   const uint4* sm;
   template <class T, int NT>
   __device__ __forceinline__ void begin(const Share<T, NT>&) {}
