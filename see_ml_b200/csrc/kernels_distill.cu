@@ -507,6 +507,7 @@ __global__ void __launch_bounds__(kSumThreads) row_loss_sum_kernel(const float* 
                                                                    const float* __restrict__ weight, size_t rows, float scale,
                                                                    float* __restrict__ loss) {
   __shared__ double part[kSumThreads / 32];
+  asm volatile("griddepcontrol.wait;" ::: "memory");     // launched while the row losses' kernel still runs
   double s = 0.0;
 #pragma unroll 4
   for (size_t r = threadIdx.x; r < rows; r += kSumThreads) {
@@ -540,7 +541,7 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
     if (many && !d.dlogits && d.vocab * elem >= (24u << 10))
-      return launch_rows<distill_stream_kernel<T, 256, 3, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a);
+      return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a);
     if (many && d.dlogits && d.vocab * elem > 4 * kMostParked)
       return launch_rows<distill_stream_kernel<T, 512, 2, true>>(d.rows, 1, false, 512 + 32, named_bytes(vecs, 512), st, a);
     const Split s = split_row(d.rows, d.vocab, elem, kMostParked);
@@ -573,8 +574,16 @@ int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
   });
 }
 int row_loss_sum(const float* row_loss, const float* weight, size_t rows, float scale, float* loss, cudaStream_t st) {
-  row_loss_sum_kernel<<<1, kSumThreads, 0, st>>>(row_loss, weight, rows, scale, loss);
-  return 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(kSumThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, row_loss_sum_kernel, row_loss, weight, rows, scale, loss) == cudaSuccess ? 1 : -1;
 }
 
 }  // namespace k

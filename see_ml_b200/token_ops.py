@@ -45,49 +45,52 @@ def _refuse(msg):
 
 
 def _matrix(name, t):
+    """Checks a matrix of logits; returns (rows, columns, row stride, dtype code, device index)."""
     if not isinstance(t, torch.Tensor) or t.dim() != 2:
         _refuse(f"{name} must be a [rows, vocab] tensor")
     if not t.is_cuda:
         _refuse(f"{name} must be device memory")
-    if t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         _refuse(f"{name} must be f32, bf16 or f16 (got {t.dtype})")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    pitch, step = t.stride()
+    if cols > 1 and step != 1:
         _refuse(f"the columns of {name} must be contiguous")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        _refuse(f"the rows of {name} overlap (row stride {t.stride(0)}, {t.shape[1]} columns)")
-    return t
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    if pitch < cols:
+        if rows > 1:
+            _refuse(f"the rows of {name} overlap (row stride {pitch}, {cols} columns)")
+        pitch = cols
+    return rows, cols, pitch, code, t.get_device()
 
 
 def _operand(name, t, shape, dtypes, device):
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or tuple(t.shape) != shape:
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
         _refuse(f"{name} must be a tensor of shape {shape}")
     if t.dtype not in dtypes:
         _refuse(f"{name} has type {t.dtype}")
-    if t.device != device:
-        _refuse(f"{name} lives on {t.device}, the logits on {device}")
+    if t.get_device() != device:
+        _refuse(f"{name} lives on {t.device}, the logits on device {device}")
     if not t.is_contiguous():
         _refuse(f"{name} must be contiguous")
     return t.data_ptr()
 
 
 def _gradient(logits, out):
+    """The gradient's tensor and its row stride."""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    _matrix("out", out)
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+    pitch = _matrix("out", out)[2]
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         _refuse("out must have the logits' shape, type and device")
-    return out
+    return out, pitch
 
 
 def _call(fn, desc, device):
-    stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream() without building its object
-    if torch.cuda.current_device() == device.index:
+    stream = torch._C._cuda_getCurrentRawStream(device)      # current_stream() without building its object
+    if torch._C._cuda_getDevice() == device:
         rc = fn(C.byref(desc), stream)
     else:
         with torch.cuda.device(device):
@@ -96,40 +99,49 @@ def _call(fn, desc, device):
         raise L.BackendError(L.last_error())
 
 
+def _teacher(teacher_id, teacher_logprob, rows, device):
+    """Checks a teacher's entries; returns (entries, token pointer, value pointer, dtype code)."""
+    if not isinstance(teacher_id, torch.Tensor) or teacher_id.dim() != 2:
+        _refuse("teacher_id must be a [rows, entries] tensor")
+    if teacher_logprob is None:
+        _refuse("teacher_logprob is missing")
+    k = teacher_id.shape[1]
+    tid = _operand("teacher_id", teacher_id, (rows, k), (_I32,), device)
+    tlp = _operand("teacher_logprob", teacher_logprob, (rows, k), _DTYPES, device)
+    return k, tid, tlp, _DTYPES[teacher_logprob.dtype]
+
+
 def token_scores(logits, labels=None, *, top_k=0, temperature=1.0, entropy=True, stats=False) -> TokenScores:
     """Log probability of `labels` (i32, negative = none), entropy and the `top_k` alternatives."""
-    _matrix("logits", logits)
-    rows, vocab = logits.shape
-    dev = logits.device
+    rows, vocab, pitch, code, dev = _matrix("logits", logits)
     if not 0 <= top_k <= min(TOP_K_MAX, vocab):
         _refuse(f"top_k must be 0..{TOP_K_MAX} and at most the vocabulary (got {top_k})")
     lab = _operand("labels", labels, (rows,), (_I32,), dev)
-    logprob = torch.empty(rows, dtype=_F32, device=dev) if labels is not None else None
-    ent = torch.empty(rows, dtype=_F32, device=dev) if entropy else None
-    st = torch.empty((rows, 2), dtype=_F32, device=dev) if stats else None
-    top_lp = torch.empty((rows, top_k), dtype=_F32, device=dev) if top_k else None
-    top_id = torch.empty((rows, top_k), dtype=_I32, device=dev) if top_k else None
-    d = L.TokenScores(logits.data_ptr(), lab, logprob.data_ptr() if logprob is not None else None,
-                      ent.data_ptr() if entropy else None, st.data_ptr() if stats else None, top_lp.data_ptr() if top_k else None,
-                      top_id.data_ptr() if top_k else None, rows, vocab, _stride(logits), _DTYPES[logits.dtype], top_k,
-                      temperature, 0)
+    where = logits.device
+    logprob = torch.empty(rows, dtype=_F32, device=where) if lab is not None else None
+    ent = torch.empty(rows, dtype=_F32, device=where) if entropy else None
+    st = torch.empty((rows, 2), dtype=_F32, device=where) if stats else None
+    top_lp = torch.empty((rows, top_k), dtype=_F32, device=where) if top_k else None
+    top_id = torch.empty((rows, top_k), dtype=_I32, device=where) if top_k else None
+    d = L.TokenScores(logits.data_ptr(), lab, logprob.data_ptr() if lab is not None else None,
+                      ent.data_ptr() if entropy else None, st.data_ptr() if stats else None,
+                      top_lp.data_ptr() if top_k else None, top_id.data_ptr() if top_k else None, rows, vocab, pitch, code,
+                      top_k, temperature, 0)
     _call(L.lib().seeml_b200_token_scores_fwd, d, dev)
     return TokenScores(logprob, ent, st, top_lp, top_id)
 
 
 def token_scores_backward(logits, labels, stats, entropy, dlogprob, dentropy, *, temperature=1.0, out=None):
     """Gradient of sum(dlogprob * logprob + dentropy * entropy); `out` may be the logits."""
-    _matrix("logits", logits)
-    rows, vocab = logits.shape
-    dev = logits.device
+    rows, vocab, pitch, code, dev = _matrix("logits", logits)
     lab = _operand("labels", labels, (rows,), (_I32,), dev)
     st = _operand("stats", stats, (rows, 2), (_F32,), dev)
     ent = _operand("entropy", entropy, (rows,), (_F32,), dev)
     dlp = _operand("dlogprob", dlogprob, (rows,), (_F32,), dev)
     dent = _operand("dentropy", dentropy, (rows,), (_F32,), dev)
-    g = _gradient(logits, out)
-    d = L.TokenScoresGrad(logits.data_ptr(), lab, st, ent, dlp, dent, g.data_ptr(), rows, vocab, _stride(logits),
-                          _stride(g), _DTYPES[logits.dtype], temperature)
+    g, g_pitch = _gradient(logits, out)
+    d = L.TokenScoresGrad(logits.data_ptr(), lab, st, ent, dlp, dent, g.data_ptr(), rows, vocab, pitch, g_pitch, code,
+                          temperature)
     _call(L.lib().seeml_b200_token_scores_bwd, d, dev)
     return g
 
@@ -138,45 +150,29 @@ def distill_topk(logits, teacher_id, teacher_logprob, *, row_weight=None, scale=
                  grad=False, saved=False, out=None) -> DistillLoss:
     """Loss against a teacher's top entries, with its gradient (`grad`, into `out` when given, which
     may be the logits) or with what `distill_topk_backward` needs (`saved`)."""
-    _matrix("logits", logits)
-    rows, vocab = logits.shape
-    dev = logits.device
-    if not isinstance(teacher_id, torch.Tensor) or teacher_id.dim() != 2:
-        _refuse("teacher_id must be a [rows, entries] tensor")
-    k = teacher_id.shape[1]
-    tid = _operand("teacher_id", teacher_id, (rows, k), (_I32,), dev)
-    tlp = _operand("teacher_logprob", teacher_logprob, (rows, k), _DTYPES, dev)
-    if tlp is None:
-        _refuse("teacher_logprob is missing")
+    rows, vocab, pitch, code, dev = _matrix("logits", logits)
+    k, tid, tlp, tcode = _teacher(teacher_id, teacher_logprob, rows, dev)
     w = _operand("row_weight", row_weight, (rows,), (_F32,), dev)
-    row_loss = torch.empty(rows, dtype=_F32, device=dev)
-    loss = torch.empty((), dtype=_F32, device=dev)
-    keep = torch.empty((rows, 4), dtype=_F32, device=dev) if saved else None
-    g = _gradient(logits, out) if grad or out is not None else None
+    where = logits.device
+    row_loss = torch.empty(rows, dtype=_F32, device=where)
+    loss = torch.empty((), dtype=_F32, device=where)
+    keep = torch.empty((rows, 4), dtype=_F32, device=where) if saved else None
+    g, g_pitch = _gradient(logits, out) if grad or out is not None else (None, vocab)
     d = L.DistillTopk(logits.data_ptr(), tid, tlp, w, row_loss.data_ptr(), loss.data_ptr(),
-                      keep.data_ptr() if saved else None, g.data_ptr() if g is not None else None, rows, vocab,
-                      _stride(logits), _stride(g) if g is not None else vocab, _DTYPES[logits.dtype],
-                      _DTYPES[teacher_logprob.dtype], k, int(bool(tail)), temperature, scale)
+                      keep.data_ptr() if saved else None, g.data_ptr() if g is not None else None, rows, vocab, pitch,
+                      g_pitch, code, tcode, k, 1 if tail else 0, temperature, scale)
     _call(L.lib().seeml_b200_distill_topk_fwd, d, dev)
     return DistillLoss(loss, row_loss, keep, g)
 
 
 def distill_topk_backward(logits, teacher_id, teacher_logprob, saved, drow_loss, *, temperature=1.0, tail=False, out=None):
     """Gradient of sum(drow_loss * row_loss) from the forward call's `saved`; `out` may be the logits."""
-    _matrix("logits", logits)
-    rows, vocab = logits.shape
-    dev = logits.device
-    if not isinstance(teacher_id, torch.Tensor) or teacher_id.dim() != 2:
-        _refuse("teacher_id must be a [rows, entries] tensor")
-    k = teacher_id.shape[1]
-    tid = _operand("teacher_id", teacher_id, (rows, k), (_I32,), dev)
-    tlp = _operand("teacher_logprob", teacher_logprob, (rows, k), _DTYPES, dev)
-    if tlp is None:
-        _refuse("teacher_logprob is missing")
+    rows, vocab, pitch, code, dev = _matrix("logits", logits)
+    k, tid, tlp, tcode = _teacher(teacher_id, teacher_logprob, rows, dev)
     sv = _operand("saved", saved, (rows, 4), (_F32,), dev)
     up = _operand("drow_loss", drow_loss, (rows,), (_F32,), dev)
-    g = _gradient(logits, out)
-    d = L.DistillTopkGrad(logits.data_ptr(), tid, tlp, sv, up, g.data_ptr(), rows, vocab, _stride(logits), _stride(g),
-                          _DTYPES[logits.dtype], _DTYPES[teacher_logprob.dtype], k, int(bool(tail)), temperature, 0)
+    g, g_pitch = _gradient(logits, out)
+    d = L.DistillTopkGrad(logits.data_ptr(), tid, tlp, sv, up, g.data_ptr(), rows, vocab, pitch, g_pitch, code, tcode, k,
+                          1 if tail else 0, temperature, 0)
     _call(L.lib().seeml_b200_distill_topk_bwd, d, dev)
     return g
