@@ -42,8 +42,8 @@ struct TopShared {
 };
 static_assert(kThreads <= 256, "a hot run's code holds the thread in 8 bits");
 // Calls f(key) for the elements of vector i whose key is at least `least` (thr: the value of that key).
-template <class T, class F>
-__device__ __forceinline__ void each_from(const Share<T, kThreads>& sh, const uint4& vec, uint32_t i, uint32_t least, float thr, F f) {
+template <class T, int NT, class F>
+__device__ __forceinline__ void each_from(const Share<T, NT>& sh, const uint4& vec, uint32_t i, uint32_t least, float thr, F f) {
   float2 e[Ty<T>::E / 2];
   Ty<T>::unpack(vec, e);
   uint32_t hit = 0;
@@ -249,14 +249,27 @@ struct Label {
   int32_t id;
   float x;
 };
-template <class T>
-__device__ __forceinline__ Label load_label(const seeml_b200_token_scores& d, size_t r, const Share<T, kThreads>& sh) {
+template <class T, int NT>
+__device__ __forceinline__ Label load_label(const seeml_b200_token_scores& d, size_t r, const Share<T, NT>& sh) {
   Label lab{-1, 0.0f};
-  if (threadIdx.x == kThreads - 1 && d.logprob) {
+  if (d.logprob) {
     lab.id = d.labels[r];
     if (lab.id >= 0) lab.x = static_cast<uint32_t>(lab.id) < sh.V ? Ty<T>::to(sh.x[lab.id]) : nan_f();
   }
   return lab;
+}
+__device__ __forceinline__ float logprob_of(float x, const Stats& row, double log_s, double inv_t) {
+  return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
+}
+__device__ __forceinline__ float label_logprob(Label lab, uint32_t V, const Stats& row, double log_s, double inv_t) {
+  return lab.id < 0 ? 0.0f : static_cast<uint32_t>(lab.id) >= V ? nan_f() : logprob_of(lab.x, row, log_s, inv_t);
+}
+__device__ __forceinline__ void write_row(const seeml_b200_token_scores& d, size_t r, const Stats& row, double log_s) {
+  if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
+  if (d.stats) {
+    d.stats[2 * r] = row.m;
+    d.stats[2 * r + 1] = row.s;
+  }
 }
 // The results of a row from its statistics and its blocks' lists of alternatives.
 __device__ __forceinline__ void write_scores(const seeml_b200_token_scores& d, size_t r, const Stats& row, Label lab,
@@ -264,18 +277,9 @@ __device__ __forceinline__ void write_scores(const seeml_b200_token_scores& d, s
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
   if (threadIdx.x >= blocks * K && threadIdx.x >= 32 && threadIdx.x < kThreads - 32) return;
   const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
-  auto logprob = [&](float x) {
-    return row.s == 0.0f ? -INFINITY : static_cast<float>((static_cast<double>(x) - row.m) * inv_t - log_s);
-  };
-  if (threadIdx.x == 0) {
-    if (d.entropy) d.entropy[r] = row.s == 0.0f ? 0.0f : static_cast<float>(log_s - static_cast<double>(row.t / row.s) * kLn2);
-    if (d.stats) {
-      d.stats[2 * r] = row.m;
-      d.stats[2 * r + 1] = row.s;
-    }
-  }
-  if (threadIdx.x == kThreads - 1 && d.logprob)
-    d.logprob[r] = lab.id < 0 ? 0.0f : static_cast<uint32_t>(lab.id) >= V ? nan_f() : logprob(lab.x);
+  auto logprob = [&](float x) { return logprob_of(x, row, log_s, inv_t); };
+  if (threadIdx.x == 0) write_row(d, r, row, log_s);
+  if (threadIdx.x == kThreads - 1 && d.logprob) d.logprob[r] = label_logprob(lab, V, row, log_s, inv_t);
   for (uint32_t i = threadIdx.x; i < blocks * K; i += kThreads) {
     const Key e = lists[i];
     if (e == 0) continue;                              // fewer than K of the block's elements reach the bound
@@ -309,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_kernel(seeml_b200_token
   if (blocks > 1) cluster_arrive(false);               // waited for ahead of the first write to another block
   if (threadIdx.x == 0) ts.hots = ts.count = 0;
   Label lab{-1, 0.0f};
-  if (rank == 0) lab = load_label(d, r, sh);           // from memory: it may lie in any block's share
+  if (rank == 0 && threadIdx.x == kThreads - 1) lab = load_label(d, r, sh);      // from memory: any block's share may hold it
   const float c = kLog2e / d.temperature;
   const Stats a = thread_stats<T, kThreads, ENT>(sh, Parked{sm}, c, nullptr, nullptr, 0);
   publish_max(ss, a.m);
@@ -361,7 +365,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   const float c = kLog2e / d.temperature;
   const uint32_t batches = sh.batches(), per_run = (batches + kSegs - 1) / kSegs;
   const Stats a = thread_stats<T, kThreads, ENT>(sh, Streamed(), c, nullptr, K ? runs : nullptr, per_run);
-  const Label lab = load_label(d, r, sh);
+  Label lab{-1, 0.0f};
+  if (threadIdx.x == kThreads - 1) lab = load_label(d, r, sh);
   // While this row's selection leaves the memory idle, the start of a row that comes next is brought into L2: 64 KiB of
   // the row three blocks per SM ahead (16384 x 32000 f32 with 16 alternatives: 371 us without, 349 us with; 128 KiB or
   // one to four blocks per SM ahead gave 356-381).
@@ -384,28 +389,194 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   write_scores(d, r, ss.block[0], lab, list, 1);
 }
 
+// Short rows: one per warp, held in registers (N vectors a lane) from the only time it is read.
+constexpr int kRowWarps = 8;
+constexpr uint32_t kRowCand = 512, kRowKeep = 192;
+// The k best of a row by k sweeps over it: what is left when more than kRowCand elements reach the bound.
+template <class T>
+__device__ __noinline__ void row_top_slow(const T* x, uint32_t V, uint32_t k, Key* out) {
+  const Share<T, 32> sh(x, 0, 0, V, 1, 0);
+  Key last = ~0ull;
+  for (uint32_t q = 0; q < k; ++q) {
+    Key best = 0;
+    for (uint32_t i = threadIdx.x; i < sh.n; i += 32)
+      each_from(sh, row_vec(sh, i), i, 0u, -INFINITY, [&](Key e) {
+        if ((q == 0 || e < last) && e > best) best = e;
+      });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const Key other = __shfl_xor_sync(0xffffffffu, best, o);
+      best = other > best ? other : best;
+    }
+    last = best;
+    if (threadIdx.x == 0) out[q] = best;
+  }
+}
+template <class T, bool ENT, int N>
+__global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml_b200_token_scores d) {
+  __shared__ __align__(16) Key cand_all[kRowWarps][kRowCand];
+  __shared__ __align__(16) Key keep_all[kRowWarps][kRowKeep];
+  __shared__ uint32_t count_all[kRowWarps];
+  const size_t r = static_cast<size_t>(blockIdx.x) * kRowWarps + threadIdx.y;
+  if (r >= d.rows) return;                             // a warp on its own from here on
+  Key* cand = cand_all[threadIdx.y];
+  uint32_t& count = count_all[threadIdx.y];
+  const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k, lane = threadIdx.x;
+  const Share<T, 32> sh(d.logits, r, d.row_stride, V, 1, 0);
+  uint4 v[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) v[q] = row_vec(sh, lane + 32 * q);
+  Label lab{-1, 0.0f};
+  if (lane == 31) lab = load_label(d, r, sh);
+  float vm[N], m = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    vm[q] = Ty<T>::vmax(v[q]);
+    m = max_nan(m, vm[q]);
+  }
+  const float c = kLog2e / d.temperature;
+  Stats row{warp_max_nan(m), 0.0f, 0.0f};
+  const float shift = row.m == -INFINITY ? 0.0f : row.m;
+#pragma unroll
+  for (int q = 0; q < N; q += kBatch) {
+    if (32 * q >= sh.n) break;
+    const uint4 part[kBatch] = {v[q], v[q + 1], v[q + 2], v[q + 3]};
+    float s, t;
+    batch_sums<T, ENT>(part, shift, c, s, t);
+    row.s += s;
+    row.t += t;
+  }
+  row.s = warp_sum(row.s);
+  row.t = ENT ? warp_sum(row.t) : 0.0f;
+  const double log_s = ln_sum(row.s), inv_t = 1.0 / static_cast<double>(d.temperature);
+  if (lane == 0) write_row(d, r, row, log_s);
+  if (lane == 31 && d.logprob) d.logprob[r] = label_logprob(lab, V, row, log_s, inv_t);
+  if (K == 0) return;
+  // the bound: as top_bound, of the vectors' maxima
+  uint32_t key[N], lo = 0xffffffffu, hi = 0, bound = 0;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    key[q] = lane + 32 * q < sh.n ? order_key(vm[q]) : 0u;
+    if (lane + 32 * q < sh.n) lo = min(lo, key[q]);
+    hi = max(hi, key[q]);
+  }
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  const uint32_t top = hi;
+  if (sh.n >= K) {
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      uint32_t at = 0;
+#pragma unroll
+      for (int q = 0; q < N; ++q) at += key[q] >= mid;
+      at = __reduce_add_sync(0xffffffffu, at);
+      if (at >= K) lo = mid;
+      else hi = mid - 1;
+      if (at >= K && at <= K + K / 2 + 2) break;
+    }
+    bound = lo;
+  }
+  if (lane == 0) count = 0;
+  __syncwarp();
+  const float thr = bound == 0 ? -INFINITY : key_value(static_cast<Key>(bound) << 32);
+#pragma unroll
+  for (int q = 0; q < N; ++q)
+    if (lane + 32 * q < sh.n && key[q] >= bound)
+      each_from(sh, v[q], lane + 32 * q, bound, thr, [&](Key e) {
+        const uint32_t p = atomicAdd(&count, 1u);
+        if (p < kRowCand) cand[p] = e;
+      });
+  __syncwarp();
+  uint32_t found = count;
+  float* lp = d.top_logprob + r * K;
+  int32_t* id = d.top_id + r * K;
+  auto put = [&](uint32_t at, Key e) {
+    id[at] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
+    lp[at] = logprob_of(key_value(e), row, log_s, inv_t);
+  };
+  if (found > kRowCand) {
+    row_top_slow(sh.x, V, K, cand);
+    __syncwarp();
+    for (uint32_t i = lane; i < K; i += 32) put(i, cand[i]);
+    return;
+  }
+  // With few vectors beside K the bound lies low. The ranking is quadratic, so the bound is raised first until few more
+  // than K of the candidates are left; equal values may not let it.
+  if (found > K + K / 4 + 16) {
+    uint32_t mine[kRowCand / 32];
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(kRowCand / 32); ++q)
+      mine[q] = lane + 32 * q < found ? static_cast<uint32_t>(cand[lane + 32 * q] >> 32) : 0u;
+    lo = max(bound, 1u);
+    hi = top;
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      uint32_t at = 0;
+#pragma unroll
+      for (int q = 0; q < static_cast<int>(kRowCand / 32); ++q) at += mine[q] >= mid;
+      at = __reduce_add_sync(0xffffffffu, at);
+      if (at >= K) lo = mid;
+      else hi = mid - 1;
+      if (at >= K && at <= K + K / 4 + 2) break;
+    }
+    uint32_t kept = 0;
+    Key* keep = keep_all[threadIdx.y];
+#pragma unroll
+    for (int q = 0; q < static_cast<int>(kRowCand / 32); ++q) {
+      const uint32_t mask = __ballot_sync(0xffffffffu, mine[q] >= lo);
+      const uint32_t at = kept + __popc(mask & ((1u << lane) - 1));
+      if (mine[q] >= lo && at < kRowKeep) keep[at] = cand[lane + 32 * q];
+      kept += __popc(mask);
+    }
+    if (kept <= kRowKeep) {
+      cand = keep;
+      found = kept;
+    }
+    __syncwarp();
+  }
+  if (lane == 0 && (found & 1u)) cand[found] = 0;      // an odd number is below the list's length
+  __syncwarp();
+  for (uint32_t i = lane; i < found; i += 32) {
+    const Key e = cand[i];
+    uint32_t ahead = 0;
+#pragma unroll 4
+    for (uint32_t j = 0; j < found; j += 2) {
+      const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(cand + j);
+      ahead += (o.x > e) + (o.y > e);
+    }
+    if (ahead < K) put(ahead, e);
+  }
+}
+
 // ---- gradient of the scores ----------------------------------------------------------------------
 // dlogits = e (a + b y) with e = 2^y, y = (x - max) log2(e) / T: the row's factors are a few numbers.
-// One block per 16 KiB of a row, four vectors in flight per thread.
-constexpr int kGradVecs = 4;
+// One block per 32 KiB of a row (one warp per 4 KiB of short rows), eight vectors in flight per thread (8192 x 32000 f32: 316 us; four vectors 356 us).
+constexpr int kGradVecs = 8;
+constexpr uint64_t kShortVecs = 1024;
 struct GradRow {
   float m, a, b;
   int32_t label;
   int skip;
 };
-template <class T>
+template <class T, int NT>
 __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_token_scores_grad d, uint32_t parts) {
   constexpr int E = Ty<T>::E;
-  __shared__ GradRow gr;
-  const size_t r = blockIdx.x / parts;
-  const uint32_t part = blockIdx.x % parts;
+  __shared__ GradRow gr_all[kThreads / NT];
+  auto sync = [] {
+    if (NT == 32) __syncwarp();
+    else __syncthreads();
+  };
+  const size_t item = static_cast<size_t>(blockIdx.x) * (kThreads / NT) + threadIdx.y, r = item / parts;
+  if (r >= d.rows) return;
+  GradRow& gr = gr_all[threadIdx.y];
+  const uint32_t part = static_cast<uint32_t>(item % parts);
   const uint32_t V = static_cast<uint32_t>(d.vocab);
-  const Share<T, kThreads> sh(d.logits, r, d.row_stride, V, parts, part);
+  const Share<T, NT> sh(d.logits, r, d.row_stride, V, parts, part);
   T* g = static_cast<T*>(d.dlogits) + r * d.grad_stride;
   uint4 v[kGradVecs];
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
-    const uint32_t i = threadIdx.x + u * kThreads;
+    const uint32_t i = threadIdx.x + u * NT;
     if (sh.whole(i)) v[u] = *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
   }
   float gl = 0.0f, gh = 0.0f, S = 0.0f, h = 0.0f, xl = 0.0f;
@@ -431,7 +602,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
       xl = Ty<T>::to(sh.x[lab]);
     }
   }
-  __syncthreads();
+  sync();
   const float2 shift = make_float2(-gr.m, -gr.m);
   const float cc = kLog2e / d.temperature;
   const float2 c = make_float2(cc, cc), a = make_float2(gr.a, gr.a), b = make_float2(gr.b, gr.b);
@@ -439,7 +610,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
   const bool same = (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
-    const uint32_t i = threadIdx.x + u * kThreads;
+    const uint32_t i = threadIdx.x + u * NT;
     if (i >= sh.n) break;
     const int j = sh.elem(i);
     const bool whole = sh.whole(i);
@@ -462,7 +633,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
     else store_elems<T>(g, j, V, f);
   }
   if (gr.label >= 0) {
-    __syncthreads();
+    sync();
     if (threadIdx.x == 0) {                    // gl (1 - p) without the cancellation, and the entropy's part
       const double inv_t = 1.0 / static_cast<double>(d.temperature);
       const double lp = (static_cast<double>(xl) - gr.m) * inv_t - log(static_cast<double>(S));
@@ -474,7 +645,22 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
 }  // namespace
 
 int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
-  const uint64_t elem = elem_bytes(d.dtype);
+  const uint64_t elem = elem_bytes(d.dtype), vecs = row_vecs(d.vocab, elem);
+  // A warp per row up to 4 KiB, and up to 8 KiB where there are many (20000 x 1000 f32: 17 us, 49 us with 16
+  // alternatives; parked by a block 75 and 141 us. x 2000: 43 and 96 us; 76 and 143 us).
+  if (vecs <= 256 || (d.rows >= kManyRows && vecs <= 512))
+    return by_type(d.dtype, [&](auto t) {
+      using T = decltype(t);
+      const dim3 grid(static_cast<unsigned>((d.rows + kRowWarps - 1) / kRowWarps)), block(32, kRowWarps);
+      if (vecs <= 256) {
+        if (d.entropy) token_scores_rows_kernel<T, true, 8><<<grid, block, 0, st>>>(d);
+        else token_scores_rows_kernel<T, false, 8><<<grid, block, 0, st>>>(d);
+      } else {
+        if (d.entropy) token_scores_rows_kernel<T, true, 16><<<grid, block, 0, st>>>(d);
+        else token_scores_rows_kernel<T, false, 16><<<grid, block, 0, st>>>(d);
+      }
+      return 1;
+    });
   // Streamed from 16 KiB a row on; below, a row parked by one block is as fast and its selection reads shared memory
   // (20000 x 3000 f32 with 16 alternatives: 137 us parked, 169 us streamed; x 8000: 184 and 189; x 16000, 10000 rows:
   // 178 and 123).
@@ -495,9 +681,14 @@ int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
 }
 int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st) {
   const uint64_t vecs = row_vecs(d.vocab, elem_bytes(d.dtype));
-  const uint32_t parts = static_cast<uint32_t>((vecs + kThreads * kGradVecs - 1) / (kThreads * kGradVecs));
+  const bool narrow = vecs <= kShortVecs;
+  const uint64_t width = (narrow ? 32 : kThreads) * kGradVecs, parts = (vecs + width - 1) / width;
+  const uint64_t per_block = narrow ? kThreads / 32 : 1;
+  const unsigned grid = static_cast<unsigned>((d.rows * parts + per_block - 1) / per_block);
   return by_type(d.dtype, [&](auto t) {
-    token_scores_grad_kernel<decltype(t)><<<static_cast<unsigned>(d.rows * parts), kThreads, 0, st>>>(d, parts);
+    using T = decltype(t);
+    if (narrow) token_scores_grad_kernel<T, 32><<<grid, dim3(32, kThreads / 32), 0, st>>>(d, static_cast<uint32_t>(parts));
+    else token_scores_grad_kernel<T, kThreads><<<grid, kThreads, 0, st>>>(d, static_cast<uint32_t>(parts));
     return 1;
   });
 }
