@@ -354,10 +354,10 @@ __global__ void __launch_bounds__(kParkThreads + 32) distill_kernel(DistillArgs 
 }
 
 // A row that one block streams: once for the loss, twice for the gradient, the second time from its end, which L2 still
-// holds when it no longer holds the start.
+// holds when it no longer holds the start; of that, `keep` batches stay in shared memory.
 template <class T, int NT, int MIN_BLOCKS, bool GRAD>
-__global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(DistillArgs a) {
-  extern __shared__ uint32_t words[];
+__global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(DistillArgs a, uint32_t keep) {
+  extern __shared__ uint4 sm[];
   __shared__ TeacherShared th;
   __shared__ StatsShared<NT> ss;
   const seeml_b200_distill_topk& d = a.d;
@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(Dis
   const size_t r = blockIdx.x;
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
   const Share<T, NT> sh(d.logits, r, d.row_stride, V, 1, 0);
+  uint32_t* words = reinterpret_cast<uint32_t*>(sm + keep * Share<T, NT>::kStep);
   T* g = GRAD ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
   const float c = kLog2e / d.temperature;
   const float w = d.row_weight ? d.row_weight[r] : 1.0f;
@@ -375,14 +376,14 @@ __global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(Dis
       return;
     }
     meet<NT + 32>();                                   // the named tokens are marked
-    const Stats mine = thread_stats<T, NT, false>(sh, Streamed(), c, words, nullptr, 0);
+    const Stats mine = thread_stats<T, NT, false>(sh, Streamed{sm, keep}, c, words, nullptr, 0);
     publish_max(ss, mine.m);
     meet<NT + 32>();
     publish_sums<false>(ss, mine, c, block_max(ss));
     meet<NT + 32>();
     if (!GRAD) return;
     meet<NT + 32>();                                   // the factors are known
-    sweep(sh, StreamedBackwards(), g, same, th.A, th.mt, c);
+    sweep(sh, StreamedBackwards{sm, keep}, g, same, th.A, th.mt, c);
     meet<NT + 32>();
     return;
   }
@@ -605,9 +606,13 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
       return 1;
     }
     if (many && !d.dlogits && d.vocab * elem >= (24u << 10))
-      return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a);
-    if (many && d.dlogits && d.vocab * elem > 4 * kMostParked)
-      return launch_rows<distill_stream_kernel<T, 512, 2, true>>(d.rows, 1, false, 512 + 32, named_bytes(vecs, 512), st, a);
+      return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a, 0u);
+    if (many && d.dlogits && d.vocab * elem > 4 * kMostParked) {
+      // two blocks share the SM's shared memory: 110 KiB each beside what they hold in any case
+      const size_t named = named_bytes(vecs, 512), batch = 512 * kBatch * 16;
+      const uint32_t keep = named < (110u << 10) ? static_cast<uint32_t>(((110u << 10) - named) / batch) : 0u;
+      return launch_rows<distill_stream_kernel<T, 512, 2, true>>(d.rows, 1, false, 512 + 32, keep * batch + named, st, a, keep);
+    }
     const Split s = split_row(d.rows, d.vocab, elem, kMostParked);
     const size_t smem = s.share * 16 + named_bytes(s.share, kParkThreads);
     return d.dlogits ? launch_rows<distill_kernel<T, true>>(d.rows, s.blocks, true, kParkThreads + 32, smem, st, a, s.share, s.blocks)

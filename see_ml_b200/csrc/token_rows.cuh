@@ -353,6 +353,8 @@ __device__ __forceinline__ void row_batch(const Share<T, NT>& sh, uint32_t b, ui
 }
 struct Streamed {
   static constexpr bool kBackwards = false;
+  uint4* kept = nullptr;                   // where the first `keep` batches stay for StreamedBackwards
+  uint32_t keep = 0;
   uint4 next[kBatch];
   template <class T, int NT>
   __device__ __forceinline__ void begin(const Share<T, NT>& sh) { row_batch(sh, 0, next); }
@@ -361,18 +363,33 @@ struct Streamed {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) v[u] = next[u];
     if (b + 1 < batches) row_batch(sh, b + 1, next);
+    if (b < keep) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) kept[b * Share<T, NT>::kStep + u * NT + threadIdx.x] = v[u];
+    }
   }
 };
-struct StreamedBackwards {               // the last batch first
+struct StreamedBackwards {                 // the last batch first, the kept ones out of shared memory
   static constexpr bool kBackwards = true;
+  const uint4* kept;
+  uint32_t keep;
   uint4 next[kBatch];
   template <class T, int NT>
-  __device__ __forceinline__ void begin(const Share<T, NT>& sh) { row_batch(sh, sh.batches() - 1, next); }
+  __device__ __forceinline__ void fetch(const Share<T, NT>& sh, uint32_t b) {
+    if (b >= keep) {
+      row_batch(sh, b, next);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) next[u] = kept[b * Share<T, NT>::kStep + u * NT + threadIdx.x];
+    }
+  }
+  template <class T, int NT>
+  __device__ __forceinline__ void begin(const Share<T, NT>& sh) { fetch(sh, sh.batches() - 1); }
   template <class T, int NT>
   __device__ __forceinline__ void batch(const Share<T, NT>& sh, uint32_t o, uint32_t batches, uint4 (&v)[kBatch]) {
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) v[u] = next[u];
-    if (o + 1 < batches) row_batch(sh, batches - 2 - o, next);
+    if (o + 1 < batches) fetch(sh, batches - 2 - o);
   }
 };
 struct Parked {
