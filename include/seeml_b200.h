@@ -184,8 +184,10 @@ int seeml_b200_xent_fwd_noalloc(const float* logits, const int32_t* labels, floa
  * All pointers are DEVICE pointers on the CURRENT device, aligned to their element, and outlive
  * the call's kernels; `stream` is a cudaStream_t (NULL = the default stream). A call only launches
  * kernels on that stream: no allocation, no synchronisation, no scratch shared between calls, so
- * calls on several streams may overlap and any of them may be captured into a graph. Results do
- * not depend on the launch: the same call gives the same bits. Arguments are checked before
+ * calls on several streams may overlap and any of them may be captured into a graph. Reductions have
+ * a fixed order: the same call gives the same bits (how a row lies in the 16-byte vectors of memory,
+ * and how many rows a call has, may move the last one). Operands other than in-place gradients do
+ * not overlap. Arguments are checked before
  * anything is launched. rows == 0 is a valid, empty call. Limits: rows <= 2^27, one row of logits
  * <= 1.5 MiB, all of them <= 2^44 bytes, top_k <= 128.
  *

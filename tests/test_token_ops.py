@@ -185,7 +185,7 @@ def test_token_scores(backend_lib, rows, V, dtype, pad, T, masked, k):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=_ids)
-@pytest.mark.parametrize("V,k", [(40, 40), (3000, 17), (32000, 128), (100003, 100)])
+@pytest.mark.parametrize("V,k", [(40, 40), (900, 100), (3000, 17), (32000, 128), (100003, 100)])
 @pytest.mark.parametrize("copies", [1, 160])
 @pytest.mark.parametrize("shape", ["constant", "ascending", "descending", "few", "one_slice", "zeros_of_both_signs", "lowest"])
 def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape, copies):
@@ -372,7 +372,7 @@ def test_gradients_against_differences(backend_lib, tail):
 
 
 @gpu
-@pytest.mark.parametrize("dtype,V", [(BF16, 4097), (F32, 1000), (F16, 32001)], ids=_ids)
+@pytest.mark.parametrize("dtype,V", [(BF16, 4097), (F32, 1000), (F16, 32001), (F32, 35003)], ids=_ids)
 @pytest.mark.parametrize("rows", [5, 300])
 @pytest.mark.parametrize("xo,go,xs,gs", [(0, 0, 0, 0), (1, 0, 3, 0), (0, 5, 0, 8), (3, 3, 7, 7), (8, 2, 1, 9)])
 def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs, rows):
@@ -422,6 +422,46 @@ def test_rows_beyond_32_bits_of_offset(backend_lib):
     _, _, grad, gerr = R.distill(_f64(flat), ids.cpu().numpy(), _f64(v), 1.0, True)
     ops.distill_topk(x, ids, v, tail=True, out=x)
     _close(x, grad, gerr, BF16, "dlogits in place")
+
+
+@gpu
+@pytest.mark.parametrize("V", [1, 3, 10])
+def test_a_million_rows_of_a_small_vocabulary(backend_lib, V):
+    """Against the same formulas in 64 bits on the device; the entries name the first and the last token. Bounds: twice
+    delta, for values up to 16."""
+    from see_ml_b200 import token_ops as ops
+    rows = 1000003
+    g = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(rows, V, generator=g, device="cuda") * 2
+    lab = torch.randint(V, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    s = ops.token_scores(x, lab, top_k=1, stats=True)
+    lp = torch.log_softmax(x.double(), 1)
+    p = lp.exp()
+    H = -(p * lp).sum(1)
+    d = R.delta(V) * 2
+    assert (s.logprob - lp.gather(1, lab.long()[:, None])[:, 0]).abs().max() <= d * 16
+    assert (s.entropy - H).abs().max() <= d * 16
+    assert torch.equal(s.top_id[:, 0].long(), x.argmax(1))
+    up = torch.ones(rows, device="cuda")
+    got = ops.token_scores_backward(x, lab, s.stats, s.entropy, up, None)
+    want = torch.zeros_like(p).scatter_(1, lab.long()[:, None], 1.0) - p
+    assert (got - want).abs().max() <= d * 16
+    ids = torch.tensor([[0, V - 1]], dtype=torch.int32, device="cuda").expand(rows, 2).contiguous()
+    q = torch.tensor([[0.5, 0.25]], device="cuda").expand(rows, 2)
+    r = ops.distill_topk(x, ids, q.log().contiguous(), tail=True, grad=True, scale=1.0, saved=True)
+    target = torch.zeros_like(p).scatter_add_(1, ids.long(), q.double())
+    named = torch.zeros_like(p, dtype=torch.bool).scatter_(1, ids.long(), True)
+    tail = torch.where(named, 0.0, p).sum(1, keepdim=True)
+    rest = 0.25 if V > 2 else 0.0                         # with every token named the tail's term is left out
+    want = p * (0.75 + rest) - target - torch.where(named, 0.0, p * rest / tail.clamp(min=1e-300))
+    assert (r.dlogits - want).abs().max() <= d * 16
+    again = ops.distill_topk_backward(x, ids, q.log().contiguous(), r.saved, up, tail=True)
+    assert (again - want).abs().max() <= d * 16
+    loss = (q.double() * (q.double().log() - lp.gather(1, ids.long()))).sum(1)
+    if V > 2:
+        loss += rest * (math.log(rest) - tail[:, 0].log())
+    assert (r.row_loss - loss).abs().max() <= d * 16
+    assert abs(r.loss.item() - loss.sum().item()) <= rows * d * 16
 
 
 @gpu
