@@ -78,7 +78,7 @@ size_t loss_scratch_doubles(size_t rows_or_elems);
 // device refused an attribute or the launch (cudaGetLastError tells).
 int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st);
 int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st);
-int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st);   // row losses, saved, dlogits
+int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st);   // row losses, saved, dlogits; loss of one row
 int distill_topk_bwd(const seeml_b200_distill_topk_grad& d, cudaStream_t st);
 // loss = scale * sum_r weight[r] * row_loss[r] in a fixed order; weight nullable, rows of weight 0 skipped
 int row_loss_sum(const float* row_loss, const float* weight, size_t rows, float scale, float* loss, cudaStream_t st);

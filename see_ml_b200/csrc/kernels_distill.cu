@@ -196,7 +196,10 @@ __device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, con
     if (e.rest > 0.0 && unnamed.s != 0.0f)
       l += e.rest * (log(e.rest) - ((static_cast<double>(unnamed.m) - all.m) * a.inv_t + ln_sum(unnamed.s) - log_s));
   }
-  d.row_loss[r] = e.bad ? nan_f() : static_cast<float>(l);
+  const float loss = e.bad ? nan_f() : static_cast<float>(l);
+  d.row_loss[r] = loss;
+  if (d.loss && d.rows == 1)             // one row needs no sum: row_loss_sum is not launched
+    *d.loss = static_cast<float>((d.row_weight ? static_cast<double>(d.row_weight[0]) : 1.0) * loss * d.scale);
   if (d.saved) {
     float* sv = d.saved + 4 * r;
     sv[0] = unnamed.m; sv[1] = unnamed.s; sv[2] = all.m; sv[3] = all.s;
@@ -204,6 +207,7 @@ __device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, con
 }
 __device__ __forceinline__ void skipped_loss(const seeml_b200_distill_topk& d, size_t r) {
   d.row_loss[r] = 0.0f;
+  if (d.loss && d.rows == 1) *d.loss = 0.0f;
   if (d.saved) {
     float* sv = d.saved + 4 * r;
     sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;

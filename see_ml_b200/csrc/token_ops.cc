@@ -191,7 +191,7 @@ int seeml_b200_distill_topk_fwd(const seeml_b200_distill_topk* d, void* stream) 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (some)
       if (int r = launched(k::distill_topk_fwd(*d, st), op)) return r;
-    if (d->loss) return launched(k::row_loss_sum(d->row_loss, d->row_weight, d->rows, d->scale, d->loss, st), op);
+    if (d->loss && d->rows != 1) return launched(k::row_loss_sum(d->row_loss, d->row_weight, d->rows, d->scale, d->loss, st), op);
     return 0;
   });
 }

@@ -81,7 +81,8 @@ def _operand(name, t, shape, dtypes, device):
 def _gradient(logits, out):
     """The gradient's tensor and its row stride."""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), logits.shape[1]
+        rows, vocab = logits.shape
+        return logits.new_empty(rows, vocab), vocab
     pitch = _matrix("out", out)[2]
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         _refuse("out must have the logits' shape, type and device")
@@ -120,9 +121,9 @@ def token_scores(logits, labels=None, *, top_k=0, temperature=1.0, entropy=True,
     where = logits.device
     logprob = torch.empty(rows, dtype=_F32, device=where) if lab is not None else None
     ent = torch.empty(rows, dtype=_F32, device=where) if entropy else None
-    st = torch.empty((rows, 2), dtype=_F32, device=where) if stats else None
-    top_lp = torch.empty((rows, top_k), dtype=_F32, device=where) if top_k else None
-    top_id = torch.empty((rows, top_k), dtype=_I32, device=where) if top_k else None
+    st = torch.empty(rows, 2, dtype=_F32, device=where) if stats else None
+    top_lp = torch.empty(rows, top_k, dtype=_F32, device=where) if top_k else None
+    top_id = torch.empty(rows, top_k, dtype=_I32, device=where) if top_k else None
     d = L.TokenScores(logits.data_ptr(), lab, logprob.data_ptr() if lab is not None else None,
                       ent.data_ptr() if entropy else None, st.data_ptr() if stats else None,
                       top_lp.data_ptr() if top_k else None, top_id.data_ptr() if top_k else None, rows, vocab, pitch, code,
@@ -155,8 +156,8 @@ def distill_topk(logits, teacher_id, teacher_logprob, *, row_weight=None, scale=
     w = _operand("row_weight", row_weight, (rows,), (_F32,), dev)
     where = logits.device
     row_loss = torch.empty(rows, dtype=_F32, device=where)
-    loss = torch.empty((), dtype=_F32, device=where)
-    keep = torch.empty((rows, 4), dtype=_F32, device=where) if saved else None
+    loss = row_loss.new_empty(())
+    keep = torch.empty(rows, 4, dtype=_F32, device=where) if saved else None
     g, g_pitch = _gradient(logits, out) if grad or out is not None else (None, vocab)
     d = L.DistillTopk(logits.data_ptr(), tid, tlp, w, row_loss.data_ptr(), loss.data_ptr(),
                       keep.data_ptr() if saved else None, g.data_ptr() if g is not None else None, rows, vocab, pitch,
