@@ -170,9 +170,10 @@ template <class T, int NT>
 __device__ __forceinline__ void store_named(T* g, const Share<T, NT>& sh, uint32_t K, const TeacherShared& th, const Entries& e,
                                             float up_t, float named, bool empty) {
   if (e.bad) return;
+  const uint32_t shift = sh.shift_to(g);
 #pragma unroll
   for (int w = 0; w < kPer; ++w) {
-    if (!((e.first >> w) & 1u) || sh.local(e.id[w]) < 0) continue;
+    if (!((e.first >> w) & 1u) || !sh.writes(e.id[w], shift)) continue;
     double q = e.q[w];
     if (e.dup) {
       q = 0.0;
@@ -233,22 +234,40 @@ __device__ __forceinline__ void load_logits(const Share<T, NT>& sh, const Entrie
   for (int w = 0; w < kPer; ++w)
     x[w] = e.id[w] >= 0 && static_cast<uint32_t>(e.id[w]) < sh.V ? Ty<T>::to(sh.x[e.id[w]]) : -INFINITY;
 }
-// Zeros over this block's share.
-template <class T, int NT>
-__device__ __forceinline__ void store_zeros(const Share<T, NT>& sh, T* g, bool same) {
-  float2 f[Ty<T>::E / 2];
-#pragma unroll
-  for (int q = 0; q < Ty<T>::E / 2; ++q) f[q] = make_float2(0.0f, 0.0f);
-  for (uint32_t i = threadIdx.x; i < sh.n; i += NT) {
-    if (same && sh.whole(i)) *reinterpret_cast<uint4*>(g + sh.elem(i)) = make_uint4(0, 0, 0, 0);
-    else store_elems<T>(g, sh.elem(i), sh.V, f);
+// The sources of a sweep: in order, and at any vector of the share (or the one behind it) once settled.
+struct ParkedSweep : Parked {
+  bool sync;                               // whether the block has not met since the copies were started
+  __device__ __forceinline__ ParkedSweep(const uint4* s, bool y) : Parked{s}, sync(y) {}
+  __device__ __forceinline__ void settle() const {
+    wait_pending(0);
+    if (sync) __syncthreads();
   }
-}
+  template <class T, int NT>
+  __device__ __forceinline__ uint4 at(const Share<T, NT>& sh, uint32_t i) const { return i < sh.n ? sm[i] : row_next(sh); }
+};
+template <class Base>
+struct StreamedSweep : Base {
+  __device__ __forceinline__ void settle() const {}
+  template <class T, int NT>
+  __device__ __forceinline__ uint4 at(const Share<T, NT>& sh, uint32_t i) const { return row_vec(sh, i); }
+};
 // The gradient of this block's share but for the named tokens.
 template <class T, int NT, class Source>
-__device__ __forceinline__ void sweep(const Share<T, NT>& sh, Source src, T* g, bool same, float A, float mt, float c) {
+__device__ __forceinline__ void sweep(const Share<T, NT>& sh, Source src, T* g, float A, float mt, float c) {
   constexpr int E = Ty<T>::E;
-  const float2 shift = make_float2(-mt, -mt), c2 = make_float2(c, c), A2 = make_float2(A, A);
+  const float2 base = make_float2(-mt, -mt), c2 = make_float2(c, c), A2 = make_float2(A, A);
+  auto grad = [&](float2 (&f)[E / 2]) {
+#pragma unroll
+    for (int q = 0; q < E / 2; ++q) {
+      const float2 y = mul2(add2(f[q], base), c2);
+      f[q] = mul2(make_float2(ex2(y.x), ex2(y.y)), A2);
+    }
+  };
+  if (const uint32_t shift = sh.shift_to(g)) {
+    src.settle();
+    sweep_shifted(sh, [&](uint32_t i) { return src.at(sh, i); }, g, shift, grad);
+    return;
+  }
   const uint32_t batches = sh.batches();
   src.begin(sh);
   for (uint32_t o = 0; o < batches; ++o) {
@@ -257,17 +276,13 @@ __device__ __forceinline__ void sweep(const Share<T, NT>& sh, Source src, T* g, 
     const uint32_t b = Source::kBackwards ? batches - 1 - o : o;
     const uint32_t i = b * Share<T, NT>::kStep + threadIdx.x;
     T* dst = g + sh.elem(i);
-    const bool fast = same && sh.whole_batch(b);
+    const bool fast = sh.whole_batch(b);
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       float2 f[E / 2];
       Ty<T>::unpack(v[u], f);
-#pragma unroll
-      for (int q = 0; q < E / 2; ++q) {
-        const float2 y = mul2(add2(f[q], shift), c2);
-        f[q] = mul2(make_float2(ex2(y.x), ex2(y.y)), A2);
-      }
-      if (fast || (same && sh.whole(i + u * NT))) *reinterpret_cast<uint4*>(dst + u * NT * E) = Ty<T>::pack(f);
+      grad(f);
+      if (fast || sh.whole(i + u * NT)) *reinterpret_cast<uint4*>(dst + u * NT * E) = Ty<T>::pack(f);
       else if (i + u * NT < sh.n) store_elems<T>(g, sh.elem(i + u * NT), sh.V, f);
     }
   }
@@ -296,9 +311,8 @@ __global__ void __launch_bounds__(kParkThreads + 32) distill_kernel(DistillArgs 
   // the row is only asked for if it counts; otherwise the whole cluster leaves
   const float w = d.row_weight ? d.row_weight[r] : 1.0f;
   if (threadIdx.x < NT) {
-    const bool same = GRAD && sh.same_phase(g);
     if (w == 0.0f) {
-      if (GRAD) store_zeros(sh, g, same);
+      if (GRAD) store_zeros(sh, g);
       return;
     }
     sh.load(sm);
@@ -314,7 +328,7 @@ __global__ void __launch_bounds__(kParkThreads + 32) distill_kernel(DistillArgs 
     if (!GRAD) return;
     meet<NT + 32>();                                   // the factors are known
     if (blocks > 1) cluster_wait();
-    sweep(sh, Parked{sm}, g, same, th.A, th.mt, c);
+    sweep(sh, ParkedSweep{sm, false}, g, th.A, th.mt, c);
     meet<NT + 32>();
     return;
   }
@@ -374,9 +388,8 @@ __global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(Dis
   const float c = kLog2e / d.temperature;
   const float w = d.row_weight ? d.row_weight[r] : 1.0f;
   if (threadIdx.x < NT) {
-    const bool same = GRAD && sh.same_phase(g);
     if (w == 0.0f) {
-      if (GRAD) store_zeros(sh, g, same);
+      if (GRAD) store_zeros(sh, g);
       return;
     }
     meet<NT + 32>();                                   // the named tokens are marked
@@ -387,7 +400,7 @@ __global__ void __launch_bounds__(NT + 32, MIN_BLOCKS) distill_stream_kernel(Dis
     meet<NT + 32>();
     if (!GRAD) return;
     meet<NT + 32>();                                   // the factors are known
-    sweep(sh, StreamedBackwards{sm, keep}, g, same, th.A, th.mt, c);
+    sweep(sh, StreamedSweep<StreamedBackwards>{{sm, keep}}, g, th.A, th.mt, c);
     meet<NT + 32>();
     return;
   }
@@ -437,14 +450,13 @@ __global__ void __launch_bounds__(32 * kRowWarps, MODE == kLoss ? 4 : 3) distill
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k;
   const Share<T, 32> sh(d.logits, r, d.row_stride, V, 1, 0);
   T* g = MODE != kLoss ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
-  const bool same = MODE != kLoss && sh.same_phase(g);
   const float c = kLog2e / d.temperature;
   const float w = MODE == kBackward ? a.upstream[r] : d.row_weight ? d.row_weight[r] : 1.0f;
   Entries e;
   float v[kPer], x[kPer];
   load_entries(d, r, e, v);
   if (w == 0.0f) {
-    if (MODE != kLoss) store_zeros(sh, g, same);
+    if (MODE != kLoss) store_zeros(sh, g);
     if (MODE != kBackward && threadIdx.x == 0) skipped_loss(d, r);
     return;
   }
@@ -470,7 +482,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, MODE == kLoss ? 4 : 3) distill
     float A, mt;
     const float named = gradient_factors(A, mt, e, up_t, unnamed, all, a);
     __syncwarp();                                      // in place: every lane has read its entries' logits
-    sweep(sh, Streamed(), g, same, A, mt, c);
+    sweep(sh, StreamedSweep<Streamed>(), g, A, mt, c);
     __syncwarp();
     store_named(g, sh, K, th, e, up_t, named, all.s == 0.0f);
   }
@@ -494,7 +506,6 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
   const bool tail = d.tail != 0;
   const Share<T, NT> sh(d.logits, r, d.row_stride, V, blocks, rank);
   T* g = static_cast<T*>(d.dlogits) + r * d.grad_stride;
-  const bool same = sh.same_phase(g);
   const float up = a.upstream[r];
   const float4 sv = load4(a.saved_in + 4 * r);
   int32_t id = -1;
@@ -505,12 +516,12 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
     if (id >= 0) v = value;
   }
   if (up == 0.0f) {
-    store_zeros(sh, g, same);
+    store_zeros(sh, g);
     return;
   }
   sh.load(sm);
-  const int at = id >= 0 && static_cast<uint32_t>(id) < V ? sh.local(id) : -1;
-  const float x = at >= 0 ? Ty<T>::to(sh.x[id]) : -INFINITY;     // only this block overwrites it
+  const bool mine = id >= 0 && static_cast<uint32_t>(id) < V && sh.writes(id, sh.shift_to(g));
+  const float x = mine ? Ty<T>::to(sh.x[id]) : -INFINITY;        // in place, only this block overwrites it
   th.id[threadIdx.x] = id;
   const float wm = warp_max_nan(v);
   if ((threadIdx.x & 31) == 0) vmax[threadIdx.x >> 5] = wm;
@@ -524,7 +535,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
   }
   th.q[threadIdx.x] = q;
   uint32_t same_id = 0;
-  if (at >= 0) {
+  if (mine) {
     const int4* id4 = reinterpret_cast<const int4*>(th.id);
 #pragma unroll 4
     for (uint32_t j = 0; 4 * j < K; ++j) {
@@ -546,7 +557,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
   const Stats unnamed{sv.x, sv.y, 0.0f}, all{sv.z, sv.w, 0.0f};
   float A, mt;
   const float named = gradient_factors(A, mt, e, up_t, unnamed, all, a);
-  sweep(sh, Parked{sm}, g, same, A, mt, kLog2e / d.temperature);
+  sweep(sh, ParkedSweep{sm, true}, g, A, mt, kLog2e / d.temperature);
   bool first = true;
   if (same_id > 1) {                                   // a token named twice: its first entry stands for all
     q = 0.0;
@@ -557,7 +568,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
       }
   }
   __syncthreads();
-  if (at >= 0 && first && !bad) {
+  if (mine && first && !bad) {
     const float ex = x == -INFINITY ? 0.0f : exp_near((static_cast<double>(x) - sv.z) * a.inv_t);
     g[id] = Ty<T>::from(all.s == 0.0f ? 0.0f : static_cast<float>(up_t * (static_cast<double>(ex) * named - q * e.inv_z)));
   }

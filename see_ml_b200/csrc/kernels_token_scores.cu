@@ -560,7 +560,7 @@ struct GradRow {
   int skip;
 };
 template <class T, int NT>
-__global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_token_scores_grad d, uint32_t parts) {
+__global__ void __launch_bounds__(kThreads, 4) token_scores_grad_kernel(seeml_b200_token_scores_grad d, uint32_t parts) {
   constexpr int E = Ty<T>::E;
   __shared__ GradRow gr_all[kThreads / NT];
   auto sync = [] {
@@ -574,11 +574,12 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
   const uint32_t V = static_cast<uint32_t>(d.vocab);
   const Share<T, NT> sh(d.logits, r, d.row_stride, V, parts, part);
   T* g = static_cast<T*>(d.dlogits) + r * d.grad_stride;
+  const uint32_t to = sh.shift_to(g);
   uint4 v[kGradVecs];
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
     const uint32_t i = threadIdx.x + u * NT;
-    if (sh.whole(i)) v[u] = *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
+    if (to == 0 && sh.whole(i)) v[u] = *reinterpret_cast<const uint4*>(sh.x + sh.elem(i));
   }
   float gl = 0.0f, gh = 0.0f, S = 0.0f, h = 0.0f, xl = 0.0f;
   if (threadIdx.x == 0) {
@@ -598,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
     gr.b = -gh * static_cast<float>(kLn2) / (S * d.temperature);
     gr.label = -1;
     // the label lies in one block's part, which reads it before it is overwritten
-    if (lab >= 0 && sh.local(lab) >= 0 && !gr.skip) {
+    if (lab >= 0 && sh.writes(lab, to) && !gr.skip) {
       gr.label = lab;
       xl = Ty<T>::to(sh.x[lab]);
     }
@@ -608,20 +609,7 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
   const float cc = kLog2e / d.temperature;
   const float2 c = make_float2(cc, cc), a = make_float2(gr.a, gr.a), b = make_float2(gr.b, gr.b);
   const bool skip = gr.skip != 0;
-  const bool same = (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == sh.phase;
-#pragma unroll
-  for (int u = 0; u < kGradVecs; ++u) {
-    const uint32_t i = threadIdx.x + u * NT;
-    if (i >= sh.n) break;
-    const int j = sh.elem(i);
-    const bool whole = sh.whole(i);
-    if (!whole) {
-      T* e = reinterpret_cast<T*>(&v[u]);
-#pragma unroll
-      for (int q = 0; q < E; ++q) e[q] = j + q >= 0 && j + q < static_cast<int>(V) ? sh.x[j + q] : Ty<T>::from(0.0f);
-    }
-    float2 f[E / 2];
-    Ty<T>::unpack(v[u], f);
+  auto grad = [&](float2 (&f)[E / 2]) {
 #pragma unroll
     for (int q = 0; q < E / 2; ++q) {
       float2 y = mul2(add2(f[q], shift), c);
@@ -630,8 +618,27 @@ __global__ void __launch_bounds__(kThreads) token_scores_grad_kernel(seeml_b200_
       f[q] = mul2(make_float2(ex2(y.x), ex2(y.y)), fma2(b, y, a));
       if (skip) f[q] = make_float2(0.0f, 0.0f);
     }
-    if (whole && same) *reinterpret_cast<uint4*>(g + j) = Ty<T>::pack(f);
-    else store_elems<T>(g, j, V, f);
+  };
+  if (to != 0) {
+    sweep_shifted(sh, [&](uint32_t i) { return i < sh.n ? row_vec(sh, i) : row_next(sh); }, g, to, grad);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kGradVecs; ++u) {
+      const uint32_t i = threadIdx.x + u * NT;
+      if (i >= sh.n) break;
+      const int j = sh.elem(i);
+      const bool whole = sh.whole(i);
+      if (!whole) {
+        T* e = reinterpret_cast<T*>(&v[u]);
+#pragma unroll
+        for (int q = 0; q < E; ++q) e[q] = j + q >= 0 && j + q < static_cast<int>(V) ? sh.x[j + q] : Ty<T>::from(0.0f);
+      }
+      float2 f[E / 2];
+      Ty<T>::unpack(v[u], f);
+      grad(f);
+      if (whole) *reinterpret_cast<uint4*>(g + j) = Ty<T>::pack(f);
+      else store_elems<T>(g, j, V, f);
+    }
   }
   if (gr.label >= 0) {
     sync();

@@ -192,10 +192,15 @@ struct Share {
     const uint32_t v = (static_cast<uint32_t>(j) + phase) / E;
     return v >= first && v - first < n ? static_cast<int>(static_cast<uint32_t>(j) + phase - first * E) : -1;
   }
+  // whether this block's sweep writes the gradient of element j, when the gradient lies `shift` on (sweep_shifted)
+  __device__ __forceinline__ bool writes(int32_t j, uint32_t shift) const {
+    const int p = j + static_cast<int>(phase) - static_cast<int>(shift);
+    return p < 0 ? first == 0 : static_cast<uint32_t>(p) / E >= first && static_cast<uint32_t>(p) / E - first < n;
+  }
   __device__ __forceinline__ uint32_t batches() const { return (n + kStep - 1) / kStep; }
-  // whether a matrix of the same type, row by row, has this row at the same place in its vectors
-  __device__ __forceinline__ bool same_phase(const T* g) const {
-    return (reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T) == phase;
+  // Where, within a vector of this row, one of the gradient's row g begins: 0 when both lie alike.
+  __device__ __forceinline__ uint32_t shift_to(const T* g) const {
+    return (phase + E - static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g) & 15u) / sizeof(T)) % E;
   }
   // the whole batch b lies inside the row
   __device__ __forceinline__ bool whole_batch(uint32_t b) const { return b * kStep >= lo && (b + 1) * kStep <= hi; }
@@ -231,6 +236,50 @@ __device__ __forceinline__ void store_elems(T* g, int j, uint32_t V, const float
 #pragma unroll
   for (int q = 0; q < Ty<T>::E; ++q)
     if (j + q >= 0 && j + q < static_cast<int>(V)) g[j + q] = Ty<T>::from(q & 1 ? f[q / 2].y : f[q / 2].x);
+}
+
+// Zeros over this block's share of the row in g.
+template <class T, int NT>
+__device__ __forceinline__ void store_zeros(const Share<T, NT>& sh, T* g) {
+  if (sh.n == 0) return;
+  constexpr uint32_t E = Ty<T>::E;
+  const uint32_t begin = static_cast<uint32_t>(max(sh.elem(0), 0)), end = static_cast<uint32_t>(min(sh.elem(sh.n), static_cast<int>(sh.V)));
+  const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(g + begin) & 15u) / sizeof(T);
+  const uint32_t body = min(begin + (off ? E - off : 0u), end), vecs = (end - body) / E, rest = body + vecs * E;
+  for (uint32_t i = threadIdx.x; i < vecs; i += NT) *reinterpret_cast<uint4*>(g + body + i * E) = make_uint4(0, 0, 0, 0);
+  for (uint32_t i = begin + threadIdx.x; i < body; i += NT) g[i] = Ty<T>::from(0.0f);
+  for (uint32_t i = rest + threadIdx.x; i < end; i += NT) g[i] = Ty<T>::from(0.0f);
+}
+// Elements [shift, E) of vector a, then [0, shift) of b.
+template <class T>
+__device__ __forceinline__ uint4 join_vectors(const uint4& a, const uint4& b, uint32_t shift) {
+  const uint32_t word = shift * sizeof(T) / 4, bits = shift * sizeof(T) % 4 * 8;
+  uint32_t w[5];
+  w[0] = word == 0 ? a.x : word == 1 ? a.y : word == 2 ? a.z : a.w;
+  w[1] = word == 0 ? a.y : word == 1 ? a.z : word == 2 ? a.w : b.x;
+  w[2] = word == 0 ? a.z : word == 1 ? a.w : word == 2 ? b.x : b.y;
+  w[3] = word == 0 ? a.w : word == 1 ? b.x : word == 2 ? b.y : b.z;
+  w[4] = word == 0 ? b.x : word == 1 ? b.y : word == 2 ? b.z : b.w;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits), __funnelshift_r(w[2], w[3], bits),
+                    __funnelshift_r(w[3], w[4], bits));
+}
+// The gradient of this block's share where the gradient's row lies otherwise in its vectors than the logits' (then it is
+// not in place): a thread takes aligned vectors of the gradient, whose logits two vectors of the row hold. vec(i) brings
+// vector i of the share, and the one behind its last; grad(f) turns logits into gradients.
+template <class T, int NT, class Vec, class Grad>
+__device__ __forceinline__ void sweep_shifted(const Share<T, NT>& sh, Vec vec, T* g, uint32_t shift, Grad grad) {
+  constexpr int E = Ty<T>::E;
+  auto one = [&](const uint4& x, int j) {
+    float2 f[E / 2];
+    Ty<T>::unpack(x, f);
+    grad(f);
+    if (j >= 0 && j + E <= static_cast<int>(sh.V)) *reinterpret_cast<uint4*>(g + j) = Ty<T>::pack(f);
+    else store_elems<T>(g, j, sh.V, f);
+  };
+  const int first = sh.elem(0) + static_cast<int>(shift);
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x; i < sh.n; i += NT) one(join_vectors<T>(vec(i), vec(i + 1), shift), first + static_cast<int>(i) * E);
+  if (sh.first == 0 && sh.n && threadIdx.x == NT - 1) one(join_vectors<T>(vec(0), vec(0), shift), first - E);      // its end is the row's start
 }
 
 __device__ __forceinline__ float warp_max_nan(float v) {
@@ -337,6 +386,16 @@ __device__ __forceinline__ uint4 row_vec(const Share<T, NT>& sh, uint32_t i) {
     for (int q = 0; q < Ty<T>::E; ++q)
       if (j + q >= 0 && j + q < static_cast<int>(sh.V)) Ty<T>::set(w, q, sh.x[j + q]);
   }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The vector behind the share's last, which is another block's: what of it lies in the row.
+template <class T, int NT>
+__device__ __forceinline__ uint4 row_next(const Share<T, NT>& sh) {
+  uint32_t w[4] = {Ty<T>::kMasked, Ty<T>::kMasked, Ty<T>::kMasked, Ty<T>::kMasked};
+  const int j = sh.elem(sh.n);
+#pragma unroll
+  for (int q = 0; q < Ty<T>::E; ++q)
+    if (j + q < static_cast<int>(sh.V)) Ty<T>::set(w, q, sh.x[j + q]);
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <class T, int NT>

@@ -384,8 +384,9 @@ def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs, rows):
     x.copy_(torch.from_numpy(rng.standard_normal((rows, V)) * 2))
     gb = torch.full((16 + rows * (V + gs),), 3.0, dtype=dtype, device="cuda")
     g = gb[go:go + rows * (V + gs)].view(rows, V + gs)[:, :V]
-    ids, v = _teacher(rng, rows, V, 9, F32)
-    lab = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    ids, v = _teacher(rng, rows, V, 128, F32)
+    lab = torch.arange(rows, dtype=torch.int32, device="cuda") * (V // rows) + torch.arange(rows, dtype=torch.int32, device="cuda") % 8
+    lab.clamp_(max=V - 1)
     one = torch.ones(rows, device="cuda")
     flat = x.contiguous()
     s0, s1 = ops.token_scores(flat, lab, top_k=9), ops.token_scores(x, lab, top_k=9, stats=True)
@@ -400,9 +401,45 @@ def test_alignments_and_strides(backend_lib, dtype, V, xo, go, xs, gs, rows):
         edge = gb.clone()
         edge[go:go + rows * (V + gs)].view(rows, V + gs)[:, :V] = 3.0
         assert (edge == 3.0).all()
-    want, err = R.scores_grad(_f64(x), np.zeros(rows, np.int32), np.ones(rows), -np.ones(rows), 1.0)
+    want, err = R.scores_grad(_f64(x), lab.cpu().numpy(), np.ones(rows), -np.ones(rows), 1.0)
     ops.token_scores_backward(x, lab, s1.stats, s1.entropy, one, -one, out=g.zero_())
     _close(g, want, err, dtype, "dlogits of the scores")
+
+
+@gpu
+@pytest.mark.parametrize("dtype,off", [(BF16, 3), (F16, 8), (F32, 1), (BF16, 0)], ids=_ids)
+@pytest.mark.parametrize("V", [17000, 70003])
+def test_every_token_once_named_and_once_the_label(backend_lib, dtype, off, V):
+    """A row per window of tokens: each token's own gradient survives whichever block writes beside it."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V)
+    K = 128
+    rows = -(-V // K)
+    xb = torch.zeros(rows * V + 16, dtype=dtype, device="cuda")
+    x = xb[off:off + rows * V].view(rows, V)
+    x.copy_(torch.randn(V, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda") * 2)
+    ids = (torch.arange(rows * K, device="cuda", dtype=torch.int32).view(rows, K)) % V
+    v = torch.full((rows, K), -math.log(K / 0.875), device="cuda")
+    p = torch.softmax(x[:1].double(), 1)
+    target = torch.zeros(rows, V, dtype=torch.float64, device="cuda").scatter_add_(1, ids.long(), v.double().exp())
+    named = torch.zeros(rows, V, dtype=torch.bool, device="cuda").scatter_(1, ids.long(), True)
+    tail = torch.where(named, 0.0, p).sum(1, keepdim=True)
+    want = p - target - torch.where(named, 0.0, 0.125 * p / tail)
+    bound = 4 * R.delta(V) * (p + 0.125 * p / tail) + 8 * R.U * target + R.half_step(dtype) * want.abs() * (1 + 2 ** -6) + R.floor_of(dtype)
+    r = ops.distill_topk(x, ids, v, tail=True, grad=True, saved=True)
+    assert ((r.dlogits - want).abs() <= bound).all()
+    g = ops.distill_topk_backward(x, ids, v, r.saved, torch.ones(rows, device="cuda"), tail=True)
+    assert ((g - want).abs() <= bound).all()
+    lab = torch.arange(rows, device="cuda", dtype=torch.int32)
+    up = torch.ones(rows, device="cuda")
+    for first in range(0, V, max(1, rows * 7)):
+        lab = (torch.arange(rows, device="cuda", dtype=torch.int32) * 7 + first) % V
+        s = ops.token_scores(x, lab, stats=True)
+        want = -p.expand(rows, -1).clone()
+        want.scatter_add_(1, lab.long()[:, None], torch.ones(rows, 1, dtype=torch.float64, device="cuda"))
+        got = ops.token_scores_backward(x, lab, s.stats, s.entropy, up, None)
+        bound = 4 * R.delta(V) * p + 4 * R.U + R.half_step(dtype) * want.abs() * (1 + 2 ** -6) + R.floor_of(dtype)
+        assert ((got - want).abs() <= bound).all()
 
 
 @gpu
