@@ -390,62 +390,112 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   write_scores(d, r, ss.block[0], lab, list, 1);
 }
 
-// Short rows: one per warp, held in registers (N vectors a lane) from the only time it is read.
+// Short rows: one per warp. Of at most N vectors a lane it is held in registers from the only time it is read; otherwise
+// (N = 0) it is streamed, and the selection goes by runs of four vectors.
 constexpr int kRowWarps = 8;
 constexpr uint32_t kRowCand = 512, kRowKeep = 192;
-// The k best of a row by k sweeps over it: what is left when more than kRowCand elements reach the bound.
+constexpr int kRowRuns = 8;                 // of a lane: rows of at most 16 KiB
+// top_overflow of one warp's row, between the keys lo and hi. Returns how many candidates are in cand (count is zero).
 template <class T>
-__device__ __noinline__ void row_top_slow(const T* x, uint32_t V, uint32_t k, Key* out) {
+__device__ __noinline__ uint32_t row_overflow(const T* x, uint32_t V, uint32_t k, uint32_t lo, uint32_t hi, Key* cand,
+                                              uint32_t* count) {
   const Share<T, 32> sh(x, 0, 0, V, 1, 0);
-  Key last = ~0ull;
-  for (uint32_t q = 0; q < k; ++q) {
-    Key best = 0;
-    for (uint32_t i = threadIdx.x; i < sh.n; i += 32)
-      each_from(sh, row_vec(sh, i), i, 0u, -INFINITY, [&](Key e) {
-        if ((q == 0 || e < last) && e > best) best = e;
-      });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Key other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
-    last = best;
-    if (threadIdx.x == 0) out[q] = best;
+  const uint32_t lane = threadIdx.x;
+  uint32_t at = ~0u;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2 + 1;
+    const float thr = key_value(static_cast<Key>(mid) << 32);
+    uint32_t c = 0;
+    for (uint32_t i = lane; i < sh.n; i += 32) each_from(sh, row_vec(sh, i), i, mid, thr, [&](Key) { ++c; });
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= k) lo = mid, at = c;
+    else hi = mid - 1;
+    if (c >= k && c <= kRowCand) break;
   }
+  const bool fits = at <= kRowCand;
+  const uint32_t least = fits ? lo : lo + 1;             // lo is below 0xffffffff unless there are k NaNs
+  if (least > lo || fits) {
+    const float thr = key_value(static_cast<Key>(least) << 32);
+    for (uint32_t i = lane; i < sh.n; i += 32)
+      each_from(sh, row_vec(sh, i), i, least, thr, [&](Key e) { cand[atomicAdd(count, 1u)] = e; });
+  }
+  __syncwarp();
+  uint32_t have = *count;
+  const float thr = key_value(static_cast<Key>(lo) << 32);
+  for (uint32_t first = 0; !fits && first < sh.n && have < k; first += 32) {
+    const uint32_t i = first + lane;
+    uint32_t mine = 0;
+    auto equal = [&](auto f) {
+      if (i < sh.n) each_from(sh, row_vec(sh, i), i, lo, thr, [&](Key e) { if (static_cast<uint32_t>(e >> 32) == lo) f(e); });
+    };
+    equal([&](Key) { ++mine; });
+    uint32_t upto = mine;                                // lanes are in the order of their vectors
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t p = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += p;
+    }
+    uint32_t pos = have + upto - mine;
+    equal([&](Key e) {
+      if (pos < k) cand[pos] = e;
+      ++pos;
+    });
+    have = min(have + __shfl_sync(0xffffffffu, upto, 31), k);
+  }
+  __syncwarp();
+  return have;
 }
 template <class T, bool ENT, int N>
 __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml_b200_token_scores d) {
   __shared__ __align__(16) Key cand_all[kRowWarps][kRowCand];
   __shared__ __align__(16) Key keep_all[kRowWarps][kRowKeep];
   __shared__ uint32_t count_all[kRowWarps];
+  constexpr int P = N ? N : kRowRuns;       // maxima of a lane
+  static_assert(kRowKeep * sizeof(Key) >= kRowRuns * 32 * sizeof(float), "the runs' maxima use keep's place before it");
   const size_t r = static_cast<size_t>(blockIdx.x) * kRowWarps + threadIdx.y;
   if (r >= d.rows) return;                             // a warp on its own from here on
   Key* cand = cand_all[threadIdx.y];
+  float* runs = reinterpret_cast<float*>(keep_all[threadIdx.y]);
   uint32_t& count = count_all[threadIdx.y];
   const uint32_t V = static_cast<uint32_t>(d.vocab), K = d.top_k, lane = threadIdx.x;
   const Share<T, 32> sh(d.logits, r, d.row_stride, V, 1, 0);
-  uint4 v[N];
-#pragma unroll
-  for (int q = 0; q < N; ++q) v[q] = row_vec(sh, lane + 32 * q);
-  Label lab{-1, 0.0f};
-  if (lane == 31) lab = load_label(d, r, sh);
-  float vm[N], m = -INFINITY;
-#pragma unroll
-  for (int q = 0; q < N; ++q) {
-    vm[q] = Ty<T>::vmax(v[q]);
-    m = max_nan(m, vm[q]);
-  }
   const float c = kLog2e / d.temperature;
-  Stats row{warp_max_nan(m), 0.0f, 0.0f};
-  const float shift = row.m == -INFINITY ? 0.0f : row.m;
+  uint4 v[N ? N : 1];
+  float vm[P];
+  Stats row;
+  Label lab{-1, 0.0f};
+  if constexpr (N != 0) {
 #pragma unroll
-  for (int q = 0; q < N; q += kBatch) {
-    if (32 * q >= sh.n) break;
-    const uint4 part[kBatch] = {v[q], v[q + 1], v[q + 2], v[q + 3]};
-    float s, t;
-    batch_sums<T, ENT>(part, shift, c, s, t);
-    row.s += s;
-    row.t += t;
+    for (int q = 0; q < N; ++q) v[q] = row_vec(sh, lane + 32 * q);
+    if (lane == 31) lab = load_label(d, r, sh);
+    float m = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      vm[q] = Ty<T>::vmax(v[q]);
+      m = max_nan(m, vm[q]);
+    }
+    row = Stats{warp_max_nan(m), 0.0f, 0.0f};
+    const float shift = row.m == -INFINITY ? 0.0f : row.m;
+#pragma unroll
+    for (int q = 0; q < N; q += kBatch) {
+      if (32 * q >= sh.n) break;
+      const uint4 part[kBatch] = {v[q], v[q + 1], v[q + 2], v[q + 3]};
+      float s, t;
+      batch_sums<T, ENT>(part, shift, c, s, t);
+      row.s += s;
+      row.t += t;
+    }
+  } else {
+    const Stats a = thread_stats<T, 32, ENT>(sh, Streamed(), c, nullptr, K ? runs : nullptr, 1);
+    if (lane == 31) lab = load_label(d, r, sh);
+    row = Stats{warp_max_nan(a.m), 0.0f, 0.0f};
+    const float y = max_nan((a.m - (row.m == -INFINITY ? 0.0f : row.m)) * c, -200.0f), f = ex2(y);
+    row.s = a.s * f;
+    row.t = ENT ? (a.t + a.s * y) * f : 0.0f;
+    if (K) {
+#pragma unroll
+      for (int q = 0; q < P; ++q) vm[q] = q < static_cast<int>(sh.batches()) ? runs[q * 32 + lane] : -INFINITY;
+    }
   }
   row.s = warp_sum(row.s);
   row.t = ENT ? warp_sum(row.t) : 0.0f;
@@ -453,23 +503,26 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
   if (lane == 0) write_row(d, r, row, log_s);
   if (lane == 31 && d.logprob) d.logprob[r] = label_logprob(lab, V, row, log_s, inv_t);
   if (K == 0) return;
-  // the bound: as top_bound, of the vectors' maxima
-  uint32_t key[N], lo = 0xffffffffu, hi = 0, bound = 0;
+  // the bound: as top_bound, of the vectors' or runs' maxima
+  constexpr uint32_t kWidth = N ? 32 : 32 * kBatch;        // vectors of the warp that one maximum per lane stands for
+  uint32_t key[P], lo = 0xffffffffu, hi = 0, bound = 0, data = 0;
 #pragma unroll
-  for (int q = 0; q < N; ++q) {
-    key[q] = lane + 32 * q < sh.n ? order_key(vm[q]) : 0u;
-    if (lane + 32 * q < sh.n) lo = min(lo, key[q]);
+  for (int q = 0; q < P; ++q) {
+    const bool some = lane + kWidth * q < sh.n;
+    key[q] = some ? order_key(vm[q]) : 0u;
+    if (some) lo = min(lo, key[q]);
     hi = max(hi, key[q]);
+    data += some;
   }
   hi = __reduce_max_sync(0xffffffffu, hi);
   const uint32_t top = hi;
-  if (sh.n >= K) {
+  if (__reduce_add_sync(0xffffffffu, data) >= K) {
     lo = __reduce_min_sync(0xffffffffu, lo);
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo) / 2 + 1;
       uint32_t at = 0;
 #pragma unroll
-      for (int q = 0; q < N; ++q) at += key[q] >= mid;
+      for (int q = 0; q < P; ++q) at += key[q] >= mid;
       at = __reduce_add_sync(0xffffffffu, at);
       if (at >= K) lo = mid;
       else hi = mid - 1;
@@ -480,13 +533,27 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
   if (lane == 0) count = 0;
   __syncwarp();
   const float thr = bound == 0 ? -INFINITY : key_value(static_cast<Key>(bound) << 32);
+  auto take = [&](Key e) {
+    const uint32_t p = atomicAdd(&count, 1u);
+    if (p < kRowCand) cand[p] = e;
+  };
+  if constexpr (N != 0) {
 #pragma unroll
-  for (int q = 0; q < N; ++q)
-    if (lane + 32 * q < sh.n && key[q] >= bound)
-      each_from(sh, v[q], lane + 32 * q, bound, thr, [&](Key e) {
-        const uint32_t p = atomicAdd(&count, 1u);
-        if (p < kRowCand) cand[p] = e;
-      });
+    for (int q = 0; q < N; ++q)
+      if (lane + 32 * q < sh.n && key[q] >= bound) each_from(sh, v[q], lane + 32 * q, bound, thr, take);
+  } else {
+#pragma unroll 1
+    for (uint32_t q = 0; q < sh.batches(); ++q) {
+      const uint32_t i = lane + kWidth * q;
+      if (i >= sh.n || order_key(runs[q * 32 + lane]) < bound) continue;
+      uint4 part[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) part[u] = row_vec(sh, i + 32 * u);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i + 32 * u < sh.n) each_from(sh, part[u], i + 32 * u, bound, thr, take);
+    }
+  }
   __syncwarp();
   uint32_t found = count;
   float* lp = d.top_logprob + r * K;
@@ -496,10 +563,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
     lp[at] = logprob_of(key_value(e), row, log_s, inv_t);
   };
   if (found > kRowCand) {
-    row_top_slow(sh.x, V, K, cand);
     __syncwarp();
-    for (uint32_t i = lane; i < K; i += 32) put(i, cand[i]);
-    return;
+    if (lane == 0) count = 0;
+    __syncwarp();
+    found = row_overflow(sh.x, V, K, bound, top, cand, &count);
   }
   // With few vectors beside K the bound lies low. The ranking is quadratic, so the bound is raised first until few more
   // than K of the candidates are left; equal values may not let it.
@@ -654,9 +721,12 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_grad_kernel(seeml_b2
 
 int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
   const uint64_t elem = elem_bytes(d.dtype), vecs = row_vecs(d.vocab, elem);
-  // A warp per row up to 4 KiB, and up to 8 KiB where there are many (20000 x 1000 f32: 17 us, 49 us with 16
-  // alternatives; parked by a block 75 and 141 us. x 2000: 43 and 96 us; 76 and 143 us).
-  if (vecs <= 256 || (d.rows >= kManyRows && vecs <= 512))
+  // A warp per row up to 4 KiB (20000 x 1000 f32: 17 us, 46 us with 16 alternatives; parked by a block 75 and 141 us), and
+  // of many rows up to 16 KiB with few alternatives, whose selection is the warp's alone: 20000 x 4000 f32 56 us without,
+  // 116 us with 16, 205 us with 64 of them, parked 79, 137 and 181 us; 746 x 4562 bf16 9 us with one, 14 us with 8,
+  // parked 11 and 12 us.
+  const uint32_t few = d.rows >= 16 * kSMs ? 16 : 2;
+  if (vecs <= 256 || (d.rows >= kManyRows && vecs <= 1024 && d.top_k <= few))
     return by_type(d.dtype, [&](auto t) {
       using T = decltype(t);
       const dim3 grid(static_cast<unsigned>((d.rows + kRowWarps - 1) / kRowWarps)), block(32, kRowWarps);
@@ -664,8 +734,8 @@ int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
         if (d.entropy) token_scores_rows_kernel<T, true, 8><<<grid, block, 0, st>>>(d);
         else token_scores_rows_kernel<T, false, 8><<<grid, block, 0, st>>>(d);
       } else {
-        if (d.entropy) token_scores_rows_kernel<T, true, 16><<<grid, block, 0, st>>>(d);
-        else token_scores_rows_kernel<T, false, 16><<<grid, block, 0, st>>>(d);
+        if (d.entropy) token_scores_rows_kernel<T, true, 0><<<grid, block, 0, st>>>(d);
+        else token_scores_rows_kernel<T, false, 0><<<grid, block, 0, st>>>(d);
       }
       return 1;
     });

@@ -185,11 +185,13 @@ def test_token_scores(backend_lib, rows, V, dtype, pad, T, masked, k):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=_ids)
-@pytest.mark.parametrize("V,k", [(40, 40), (900, 100), (3000, 17), (32000, 128), (100003, 100)])
-@pytest.mark.parametrize("copies", [1, 160])
+@pytest.mark.parametrize("V,k", [(40, 40), (900, 100), (1900, 128), (3000, 16), (32000, 128), (100003, 100)])
+@pytest.mark.parametrize("copies", [1, 160, 1200])
 @pytest.mark.parametrize("shape", ["constant", "ascending", "descending", "few", "one_slice", "zeros_of_both_signs", "lowest"])
 def test_top_alternatives_of_awkward_rows(backend_lib, dtype, V, k, shape, copies):
     """Ties go to the lower index, whatever the order and wherever the great values lie."""
+    if copies * V > 20000000:
+        pytest.skip("more than this adds nothing: calls of so many long rows go the way of 160 copies")
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(V + k)
     j = np.arange(V)
