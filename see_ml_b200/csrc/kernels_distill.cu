@@ -603,6 +603,7 @@ DistillArgs distill_args(const seeml_b200_distill_topk& d) {
 }
 // Bytes of the words that mark the named tokens of a share.
 size_t named_bytes(uint64_t vecs, int threads) { return (vecs + kBatch * threads - 1) / (kBatch * threads) * threads * 4; }
+// Of a row in one block: six blocks live on an SM (16384 x 32000 f32, step: 700 us; 66 KiB and three blocks 756 us).
 constexpr uint64_t kMostParked = 34u << 10;
 
 }  // namespace
@@ -620,9 +621,14 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
       else distill_rows_kernel<T, kLoss><<<grid, dim3(32, kRowWarps), 0, st>>>(a);
       return 1;
     }
-    if (many && !d.dlogits && d.vocab * elem >= (24u << 10))
+    // The loss of rows that one block does not hold is streamed: 18181 x 8444 f32 157 us, parked 143; 16666 x 9212
+    // 148 and 163; 6000 x 51198 bf16 121 and 174.
+    if (many && !d.dlogits && d.vocab * elem > kMostParked)
       return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a, 0u);
-    if (many && d.dlogits && d.vocab * elem > 4 * kMostParked) {
+    // The step streams a row twice where parking it takes more than four blocks, or sixteen of four-byte logits, which
+    // have half the arithmetic to a byte: 16666 x 46078 bf16 820 us, parked 798; 8333 x 92158 bf16 728 and 812; 1500 x
+    // 511998 bf16 984 and 1742; 6250 x 61436 f32 587 and 579; 3000 x 127996 f32 886 and 663; 1500 x 255999 f32 966 and 1357.
+    if (many && d.dlogits && d.vocab * elem > (elem == 2 ? 4 : 16) * kMostParked) {
       // two blocks share the SM's shared memory: 110 KiB each beside what they hold in any case
       const size_t named = named_bytes(vecs, 512), batch = 512 * kBatch * 16;
       const uint32_t keep = named < (110u << 10) ? static_cast<uint32_t>(((110u << 10) - named) / batch) : 0u;

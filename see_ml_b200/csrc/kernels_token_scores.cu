@@ -618,9 +618,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
 
 // ---- gradient of the scores ----------------------------------------------------------------------
 // dlogits = e (a + b y) with e = 2^y, y = (x - max) log2(e) / T: the row's factors are a few numbers.
-// One block per 32 KiB of a row (one warp per 4 KiB of short rows), eight vectors in flight per thread (8192 x 32000 f32: 316 us; four vectors 356 us).
+// One block per 32 KiB of a row or one warp per 4 KiB, eight vectors in flight per thread (8192 x 32000 f32: 316 us; four vectors 356 us).
 constexpr int kGradVecs = 8;
-constexpr uint64_t kShortVecs = 1024;
 struct GradRow {
   float m, a, b;
   int32_t label;
@@ -739,17 +738,17 @@ int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
       }
       return 1;
     });
-  // Streamed from 16 KiB a row on; below, a row parked by one block is as fast and its selection reads shared memory
-  // (20000 x 3000 f32 with 16 alternatives: 137 us parked, 169 us streamed; x 8000: 184 and 189; x 16000, 10000 rows:
-  // 178 and 123).
-  if (d.rows >= kManyRows && d.vocab * elem >= (24u << 10))
+  // Longer rows are streamed, of four-byte logits from 28 KiB on, below which a row parked by one block is as fast and its
+  // selection reads shared memory (8 alternatives: 23076 x 6652 f32 209 us streamed, 181 parked; x 7676, 20000 rows: 184
+  // and 179; x 12284, 12500 rows: 134 and 156; 33333 x 9214 bf16 364 and 370; 8333 x 36862 bf16 144 and 271).
+  if (d.rows >= kManyRows && d.vocab * elem > (elem == 2 ? 16u : 28u) << 10)
     return by_type(d.dtype, [&](auto t) {
       using T = decltype(t);
       if (d.entropy) token_scores_stream_kernel<T, true><<<static_cast<unsigned>(d.rows), kThreads, 0, st>>>(d);
       else token_scores_stream_kernel<T, false><<<static_cast<unsigned>(d.rows), kThreads, 0, st>>>(d);
       return 1;
     });
-  const Split s = split_row(d.rows, d.vocab, elem, 66u << 10);
+  const Split s = split_row(d.rows, d.vocab, elem, 66u << 10);      // three blocks an SM
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
     const size_t smem = s.share * 16 + sizeof(Key) * s.blocks * d.top_k;
@@ -759,7 +758,10 @@ int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
 }
 int token_scores_bwd(const seeml_b200_token_scores_grad& d, cudaStream_t st) {
   const uint64_t vecs = row_vecs(d.vocab, elem_bytes(d.dtype));
-  const bool narrow = vecs <= kShortVecs;
+  // Parts of a row go to warps of which eight share a block, or of few rows to blocks of their own, whose threads read
+  // less of what a row has: 50000 x 3068 f32 186 us by warps, 284 by blocks; 4096 x 65537 bf16 174 and 182; 600 x 4000 f32
+  // 6.0 and 6.7; 296 x 32000 f32 11.8 and 11.4; 64 x 1000 f32 5.1 and 3.9.
+  const bool narrow = d.rows >= 4 * kSMs;
   const uint64_t width = (narrow ? 32 : kThreads) * kGradVecs, parts = (vecs + width - 1) / width;
   const uint64_t per_block = narrow ? kThreads / 32 : 1;
   const unsigned grid = static_cast<unsigned>((d.rows * parts + per_block - 1) / per_block);

@@ -301,7 +301,7 @@ def test_distill(backend_lib, rows, V, dtype, pad, T, masked, K, tail, tdtype):
 @gpu
 @pytest.mark.parametrize("copies", [1, 30])
 @pytest.mark.parametrize("tail", [False, True])
-@pytest.mark.parametrize("V", [9, 3000, 70001])
+@pytest.mark.parametrize("V", [9, 3000, 70001, 140003])
 def test_distill_of_awkward_rows(backend_lib, V, tail, copies):
     from see_ml_b200 import token_ops as ops
     rng = np.random.default_rng(V)
@@ -442,6 +442,31 @@ def test_every_token_once_named_and_once_the_label(backend_lib, dtype, off, V):
         got = ops.token_scores_backward(x, lab, s.stats, s.entropy, up, None)
         bound = 4 * R.delta(V) * p + 4 * R.U + R.half_step(dtype) * want.abs() * (1 + 2 ** -6) + R.floor_of(dtype)
         assert ((got - want).abs() <= bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,off", [(BF16, 3), (F16, 8), (F32, 1), (F32, 0)], ids=_ids)
+@pytest.mark.parametrize("V", [40, 4500])
+def test_scores_gradient_of_many_rows(backend_lib, dtype, off, V):
+    """Every token once the label, in as many rows; rows without an upstream gradient among them."""
+    from see_ml_b200 import token_ops as ops
+    rows = max(V, 1000)
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    xb = torch.zeros(rows * V + 16, dtype=dtype, device="cuda")
+    x = xb[off:off + rows * V].view(rows, V)
+    x.copy_(torch.randn(rows, V, generator=gen, device="cuda") * 2)
+    lab = torch.arange(rows, device="cuda", dtype=torch.int32) % V
+    gl = torch.randn(rows, generator=gen, device="cuda")
+    gl[::7] = 0.0
+    s = ops.token_scores(x, lab, stats=True)
+    p = torch.softmax(x.double(), 1)
+    one = torch.zeros_like(p).scatter_(1, lab.long()[:, None], 1.0)
+    want = gl.double()[:, None] * (one - p)
+    bound = gl.double().abs()[:, None] * (4 * R.delta(V) * p + 4 * R.U * one) + R.half_step(dtype) * want.abs() * (1 + 2 ** -6) + R.floor_of(dtype)
+    got = ops.token_scores_backward(x, lab, s.stats, s.entropy, gl, None)
+    assert ((got - want).abs() <= bound).all()
+    inplace = ops.token_scores_backward(x, lab, s.stats, s.entropy, gl, None, out=x)
+    assert inplace is x and torch.equal(x, got) and (xb[:off] == 0).all() and (xb[off + rows * V:] == 0).all()
 
 
 @gpu
