@@ -625,10 +625,10 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
     // 148 and 163; 6000 x 51198 bf16 121 and 174.
     if (many && !d.dlogits && d.vocab * elem > kMostParked)
       return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a, 0u);
-    // The step streams a row twice where parking it takes more than four blocks, or sixteen of four-byte logits, which
-    // have half the arithmetic to a byte: 16666 x 46078 bf16 820 us, parked 798; 8333 x 92158 bf16 728 and 812; 1500 x
+    // The step streams a row twice where parking it takes more than four blocks. Four-byte logits, which have half the
+    // arithmetic to a byte, are parked until eight blocks would hold more than twice as much each: 16666 x 46078 bf16 820 us, parked 798; 8333 x 92158 bf16 728 and 812; 1500 x
     // 511998 bf16 984 and 1742; 6250 x 61436 f32 587 and 579; 3000 x 127996 f32 886 and 663; 1500 x 255999 f32 966 and 1357.
-    if (many && d.dlogits && d.vocab * elem > (elem == 2 ? 4 : 16) * kMostParked) {
+    if (many && d.dlogits && d.vocab * elem > (elem == 2 ? 4 : 2 * kClusterMax) * kMostParked) {
       // two blocks share the SM's shared memory: 110 KiB each beside what they hold in any case
       const size_t named = named_bytes(vecs, 512), batch = 512 * kBatch * 16;
       const uint32_t keep = named < (110u << 10) ? static_cast<uint32_t>(((110u << 10) - named) / batch) : 0u;
