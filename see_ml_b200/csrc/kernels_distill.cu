@@ -614,7 +614,7 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
   const bool many = d.rows >= kManyRows;
   return by_type(d.dtype, [&](auto t) {
     using T = decltype(t);
-    // 20000 x 4000 f32: loss 73 us, 94 parked by a block; x 3000: with the gradient 121 us and 130, x 4000 160 and 138
+    // 20000 x 4000 f32: loss 71 us, 88 parked by a block; x 3000: with the gradient 118 us and 128, x 4000 156 and 135
     if (many && vecs * 16 <= (d.dlogits ? 12u << 10 : kShortRow)) {
       const unsigned grid = static_cast<unsigned>((d.rows + kRowWarps - 1) / kRowWarps);
       if (d.dlogits) distill_rows_kernel<T, kStep><<<grid, dim3(32, kRowWarps), 0, st>>>(a);
@@ -626,8 +626,9 @@ int distill_topk_fwd(const seeml_b200_distill_topk& d, cudaStream_t st) {
     if (many && !d.dlogits && d.vocab * elem > kMostParked)
       return launch_rows<distill_stream_kernel<T, 256, 4, false>>(d.rows, 1, false, 256 + 32, named_bytes(vecs, 256), st, a, 0u);
     // The step streams a row twice where parking it takes more than four blocks. Four-byte logits, which have half the
-    // arithmetic to a byte, are parked until eight blocks would hold more than twice as much each: 16666 x 46078 bf16 820 us, parked 798; 8333 x 92158 bf16 728 and 812; 1500 x
-    // 511998 bf16 984 and 1742; 6250 x 61436 f32 587 and 579; 3000 x 127996 f32 886 and 663; 1500 x 255999 f32 966 and 1357.
+    // arithmetic to a byte, are parked until eight blocks would hold more than twice as much each: 16666 x 46078 bf16
+    // 820 us, parked 798; 8333 x 92158 bf16 728 and 812; 1500 x 511998 bf16 984 and 1742; 8333 x 46076 f32 655 and 615;
+    // 3000 x 127996 f32 886 and 663; 1500 x 255999 f32 966 and 1357.
     if (many && d.dlogits && d.vocab * elem > (elem == 2 ? 4 : 2 * kClusterMax) * kMostParked) {
       // two blocks share the SM's shared memory: 110 KiB each beside what they hold in any case
       const size_t named = named_bytes(vecs, 512), batch = 512 * kBatch * 16;
@@ -660,7 +661,7 @@ int distill_topk_bwd(const seeml_b200_distill_topk_grad& b, cudaStream_t st) {
   a.saved_in = b.saved;
   a.upstream = b.drow_loss;
   return by_type(b.dtype, [&](auto t) {
-    // 20000 x 1000 f32: 42 us, 65 parked by a block; x 2000: 66 and 69, x 3000: 92 and 85
+    // 20000 x 1000 f32: 43 us, 60 by a block; x 2000: 66 and 65, x 3000: 90 and 79
     if (b.rows >= kManyRows && row_vecs(b.vocab, elem_bytes(b.dtype)) * 16 <= (8u << 10)) {
       const unsigned grid = static_cast<unsigned>((b.rows + kRowWarps - 1) / kRowWarps);
       distill_rows_kernel<decltype(t), kBackward><<<grid, dim3(32, kRowWarps), 0, st>>>(a);

@@ -618,7 +618,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
 
 // ---- gradient of the scores ----------------------------------------------------------------------
 // dlogits = e (a + b y) with e = 2^y, y = (x - max) log2(e) / T: the row's factors are a few numbers.
-// One block per 32 KiB of a row or one warp per 4 KiB, eight vectors in flight per thread (8192 x 32000 f32: 316 us; four vectors 356 us).
+// One block per 32 KiB of a row or one warp per 4 KiB, eight vectors in flight per thread (8192 x 32000 f32: 304 us; four
+// vectors 361 us).
 constexpr int kGradVecs = 8;
 struct GradRow {
   float m, a, b;
@@ -720,9 +721,9 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_grad_kernel(seeml_b2
 
 int token_scores_fwd(const seeml_b200_token_scores& d, cudaStream_t st) {
   const uint64_t elem = elem_bytes(d.dtype), vecs = row_vecs(d.vocab, elem);
-  // A warp per row up to 4 KiB (20000 x 1000 f32: 17 us, 46 us with 16 alternatives; parked by a block 75 and 141 us), and
+  // A warp per row up to 4 KiB (20000 x 1000 f32: 17 us, 48 us with 16 alternatives; parked by a block 74 and 141 us), and
   // of many rows up to 16 KiB with few alternatives, whose selection is the warp's alone: 20000 x 4000 f32 56 us without,
-  // 116 us with 16, 205 us with 64 of them, parked 79, 137 and 181 us; 746 x 4562 bf16 9 us with one, 14 us with 8,
+  // 115 us with 16, 205 us with 64 of them, parked 79, 138 and 181 us; 746 x 4562 bf16 9 us with one, 14 us with 8,
   // parked 11 and 12 us.
   const uint32_t few = d.rows >= 16 * kSMs ? 16 : 2;
   if (vecs <= 256 || (d.rows >= kManyRows && vecs <= 1024 && d.top_k <= few))
