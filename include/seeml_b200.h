@@ -247,7 +247,7 @@ int seeml_b200_token_scores_bwd(const seeml_b200_token_scores_grad* d, void* str
  *   row_loss[r] = l,   loss = scale * sum_r row_weight[r] * row_loss[r]
  * (there is no T^2; put it into scale). With dlogits the gradient of `loss` with respect to the
  * logits is written in the same pass, in the logits' type; dlogits may be the logits themselves.
- * A row of weight 0 is not read: row_loss 0, gradient 0. A token named twice counts with the sum
+ * A row of weight 0 is skipped, its logits are not read: row_loss 0, gradient 0. A token named twice counts with the sum
  * of its entries' q. An entry with a token >= vocab is not dereferenced; it makes the row NaN. */
 typedef struct seeml_b200_distill_topk {
   const void* logits;
@@ -256,7 +256,7 @@ typedef struct seeml_b200_distill_topk {
   const float* row_weight;       /* [rows]; NULL = ones */
   float* row_loss;               /* [rows] */
   float* loss;                   /* scalar; may be NULL */
-  float* saved;                  /* [rows, 4]: max and exp sum over unnamed tokens, over all; may be NULL */
+  float* saved;                  /* [rows, 4]: max and exp sum over unnamed tokens, over all (zeros: skipped); may be NULL */
   void* dlogits;                 /* may be NULL; row r at dlogits + r * grad_stride elements */
   uint64_t rows, vocab, row_stride, grad_stride;
   uint32_t dtype, teacher_dtype, top_k, tail;
@@ -265,8 +265,8 @@ typedef struct seeml_b200_distill_topk {
 int seeml_b200_distill_topk_fwd(const seeml_b200_distill_topk* d, void* stream);
 
 /* Gradient of sum_r drow_loss[r] * row_loss[r] with respect to the logits, from `saved` of the
- * forward call. A row whose drow_loss is 0 gets zeros and is not read. dlogits may be the logits
- * themselves; any other overlap is refused. */
+ * forward call. A row whose drow_loss is 0, or that the forward call skipped, gets zeros and its
+ * logits are not read. dlogits may be the logits themselves; any other overlap is refused. */
 typedef struct seeml_b200_distill_topk_grad {
   const void* logits;
   const int32_t* teacher_id;

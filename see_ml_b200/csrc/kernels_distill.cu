@@ -211,9 +211,12 @@ __device__ __forceinline__ void skipped_loss(const seeml_b200_distill_topk& d, s
   if (d.loss && d.rows == 1) *d.loss = 0.0f;
   if (d.saved) {
     float* sv = d.saved + 4 * r;
-    sv[0] = -INFINITY; sv[1] = 0.0f; sv[2] = -INFINITY; sv[3] = 0.0f;
+    sv[0] = sv[1] = sv[2] = sv[3] = 0.0f;
   }
 }
+// Whether the forward call skipped the row: no other has a sum of 0 under a finite maximum. Its loss is 0 whatever its
+// logits and entries, so they are not looked at here either (without sums to go by, an exponential may be infinite).
+__device__ __forceinline__ bool was_skipped(const float4& saved) { return saved.w == 0.0f && saved.z == 0.0f; }
 // The entry warp: the words of thread_stats that leave the named tokens out, n bytes at 16.
 template <class T, int NT>
 __device__ __forceinline__ void mark_named(uint32_t* words, uint32_t bytes, const Entries& e, const Share<T, NT>& sh) {
@@ -452,10 +455,11 @@ __global__ void __launch_bounds__(32 * kRowWarps, MODE == kLoss ? 4 : 3) distill
   T* g = MODE != kLoss ? static_cast<T*>(d.dlogits) + r * d.grad_stride : nullptr;
   const float c = kLog2e / d.temperature;
   const float w = MODE == kBackward ? a.upstream[r] : d.row_weight ? d.row_weight[r] : 1.0f;
+  const float4 sv = MODE == kBackward ? load4(a.saved_in + 4 * r) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   Entries e;
   float v[kPer], x[kPer];
   load_entries(d, r, e, v);
-  if (w == 0.0f) {
+  if (w == 0.0f || (MODE == kBackward && was_skipped(sv))) {
     if (MODE != kLoss) store_zeros(sh, g);
     if (MODE != kBackward && threadIdx.x == 0) skipped_loss(d, r);
     return;
@@ -471,7 +475,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, MODE == kLoss ? 4 : 3) distill
   }
   entries_exp(V, K, d.tail != 0, a.inv_t, v, x, th, e);
   if (MODE == kBackward) {
-    const float4 sv = load4(a.saved_in + 4 * r);
     unnamed = Stats{sv.x, sv.y, 0.0f};
     all = Stats{sv.z, sv.w, 0.0f};
   } else {
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(kGradThreads) distill_grad_kernel(DistillArgs 
     const float value = load_as_f32(d.teacher_logprob, d.teacher_dtype, r * K + threadIdx.x);
     if (id >= 0) v = value;
   }
-  if (up == 0.0f) {
+  if (up == 0.0f || was_skipped(sv)) {
     store_zeros(sh, g);
     return;
   }

@@ -611,3 +611,28 @@ def test_streams_and_graphs_give_the_same_bits(backend_lib, rows):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(want[1], outs[0]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V", [(F32, 40), (BF16, 700), (F16, 3001), (F32, 20003), (BF16, 140003)], ids=_ids)
+@pytest.mark.parametrize("copies", [1, 100])
+@pytest.mark.parametrize("tail", [False, True])
+def test_backward_of_rows_that_the_forward_call_skipped(backend_lib, dtype, V, copies, tail):
+    """A row of weight 0 has a loss of 0 whatever its logits and entries, so its gradient is 0 whatever comes from above."""
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((3, V))
+    x[0] += 200.0                     # exp(x / T) is beyond f32
+    x[1, 1], x[1, 2] = np.nan, np.inf
+    t = torch.from_numpy(x).to(dtype).cuda()
+    ids, v = _teacher(rng, 3, V, 5, F32)
+    ids[1, 0] = V                     # beyond the vocabulary
+    w, up = torch.tensor([0.0, 0.0, 1.0], device="cuda"), torch.tensor([1.0, -2.0, 3.0], device="cuda")
+    _, _, grad, gerr = R.distill(_f64(t)[2:], ids.cpu().numpy()[2:], _f64(v)[2:], 0.5, tail)
+    many = [a.repeat(copies, *[1] * (a.dim() - 1)) for a in (t, ids, v, w, up)]
+    r = ops.distill_topk(*many[:3], row_weight=many[3], temperature=0.5, tail=tail, saved=True)
+    for out in (None, torch.empty(3 * copies, V + 1, dtype=dtype, device="cuda")[:, 1:]):
+        g = ops.distill_topk_backward(*many[:3], r.saved, many[4], temperature=0.5, tail=tail, out=out).view(copies, 3, V)
+        assert (g[:, :2] == 0).all()
+        for c in {0, copies // 2, copies - 1}:
+            _close(g[c, 2:], 3.0 * grad, 3.0 * gerr, dtype, "dlogits of a row that counted")
