@@ -187,7 +187,9 @@ __device__ __forceinline__ void store_named(T* g, const Share<T, NT>& sh, uint32
 __device__ __forceinline__ void distill_loss(const DistillArgs& a, size_t r, const Entries& e, const Stats& unnamed, const Stats& all) {
   const seeml_b200_distill_topk& d = a.d;
   double l = 0.0;
-  if (all.s == 0.0f) {                   // nothing left of the student's row
+  if (all.s != all.s) {                  // a NaN or +inf among the logits, also of tokens that the teacher does not want
+    l = all.s;
+  } else if (all.s == 0.0f) {            // nothing left of the student's row
     if (e.qsum != 0.0) l = INFINITY;
   } else {
     const double log_s = ln_sum(all.s);

@@ -636,3 +636,25 @@ def test_backward_of_rows_that_the_forward_call_skipped(backend_lib, dtype, V, c
         assert (g[:, :2] == 0).all()
         for c in {0, copies // 2, copies - 1}:
             _close(g[c, 2:], 3.0 * grad, 3.0 * gerr, dtype, "dlogits of a row that counted")
+
+
+@gpu
+@pytest.mark.parametrize("rows,V", [(6, 9), (6, 3000), (6, 140003), (300, 9), (300, 3500), (300, 30000), (300, 140003)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_row_that_is_not_finite_has_no_loss_without_a_teacher_either(backend_lib, rows, V, tail):
+    """Entries that are absent, or without mass, leave neither the loss nor the gradient of such a row finite."""
+    from see_ml_b200 import token_ops as ops
+    x = torch.zeros(rows, V, device="cuda")
+    x[0::6, 3], x[1::6, 4], x[2::6, 0] = math.nan, math.inf, math.nan
+    ids = torch.full((rows, 2), -1, dtype=torch.int32, device="cuda")
+    ids[2::6, 1] = ids[3::6, 0] = 0                           # the token itself, named without mass
+    v = torch.full((rows, 2), -math.inf, device="cuda")
+    r = ops.distill_topk(x, ids, v, tail=tail, grad=True, saved=True)
+    alone = ops.distill_topk(x, ids, v, tail=tail)
+    g = ops.distill_topk_backward(x, ids, v, r.saved, torch.ones(rows, device="cuda"), tail=tail)
+    lost = torch.arange(rows, device="cuda") % 6 < 3
+    for loss in (r.row_loss, alone.row_loss):
+        assert loss[lost].isnan().all() and loss[~lost].isfinite().all()
+    assert r.loss.isnan() and alone.loss.isnan()
+    for d in (r.dlogits, g):
+        assert d[lost].isnan().all() and d[~lost].isfinite().all()
