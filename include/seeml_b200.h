@@ -189,7 +189,8 @@ int seeml_b200_xent_fwd_noalloc(const float* logits, const int32_t* labels, floa
  * and how many rows a call has, may move the last one). Operands other than in-place gradients do
  * not overlap. Arguments are checked before
  * anything is launched. rows == 0 is a valid, empty call. Limits: rows <= 2^27, one row of logits
- * <= 1.5 MiB, all of them <= 2^44 bytes, top_k <= 128.
+ * <= 1.5 MiB, all of them <= 2^44 bytes, top_k <= 128, temperatures finite and >= 1e-30; what comes
+ * from above, over the temperature (dlogprob / T, scale * row_weight / T, ...), stays within f32.
  *
  * x is a row of logits, T the temperature, p = softmax(x / T). A logit of -inf is a masked token
  * (p = 0). A row that is masked as a whole has log probabilities of -inf, entropy 0 and a zero
@@ -198,6 +199,7 @@ int seeml_b200_xent_fwd_noalloc(const float* logits, const int32_t* labels, floa
 #define SEEML_B200_DTYPE_BF16 1u
 #define SEEML_B200_DTYPE_F16 2u
 #define SEEML_B200_TOP_K_MAX 128u
+#define SEEML_B200_TEMPERATURE_MIN 1e-30f
 
 /* Token scores: of each row the log probability of one given token, the entropy of p, and the
  * top_k most likely tokens with their log probabilities (greater logit first, ties and masked

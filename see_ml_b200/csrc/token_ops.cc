@@ -69,8 +69,8 @@ int check_matrix(const char* op, uint64_t rows, uint64_t vocab, uint64_t stride,
   if (rows * (vocab * elem_bytes(dtype)) > kMaxBytes) return fail(unit + "more than 2^44 bytes of logits");
   if (stride < vocab || stride > kMaxElems / (rows ? rows : 1))
     return fail(unit + "row stride " + std::to_string(stride) + " is below vocab or beyond the address space");
-  if (!(temperature > 0.0f) || std::isinf(temperature) || std::isinf(1.0f / temperature))
-    return fail(unit + "temperature must be positive and finite");
+  if (!(temperature >= SEEML_B200_TEMPERATURE_MIN) || std::isinf(temperature))
+    return fail(unit + "temperature must be finite and at least 1e-30");
   return 0;
 }
 

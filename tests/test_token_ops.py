@@ -658,3 +658,49 @@ def test_row_that_is_not_finite_has_no_loss_without_a_teacher_either(backend_lib
     assert r.loss.isnan() and alone.loss.isnan()
     for d in (r.dlogits, g):
         assert d[lost].isnan().all() and d[~lost].isfinite().all()
+
+
+COLD = np.float32(1e-30)                                      # the lowest temperature that is taken
+
+
+@pytest.mark.parametrize("fn,make", [("seeml_b200_token_scores_fwd", _scores), ("seeml_b200_token_scores_bwd", _scores_grad),
+                                     ("seeml_b200_distill_topk_fwd", _distill), ("seeml_b200_distill_topk_bwd", _distill_grad)],
+                         ids=lambda v: v.replace("seeml_b200_", "") if isinstance(v, str) else "")
+def test_temperatures_next_to_the_lowest(backend_lib, fn, make):
+    """Below it log2(e) / T and the gradients' factors leave f32; 3.5e-39 has a finite 1 / T and no finite log2(e) / T."""
+    for t in (np.nextafter(COLD, np.float32(0)), 3.5e-39, 1e-38):
+        rc, err = _rc(fn, make(temperature=t))
+        assert rc != 0 and "temperature" in err, (t, err)
+    for t in (COLD, 3e38):
+        assert _rc(fn, make(temperature=t, rows=0, **({"loss": None} if make is _distill else {})))[0] == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [2, 400])
+def test_the_lowest_temperature(backend_lib, rows):
+    """p is 1 / 2 on the two greatest tokens and 0 elsewhere, exactly; gradients are those of T = 1 over T."""
+    from see_ml_b200 import token_ops as ops
+    V, T = 5000, float(COLD)
+    x = torch.zeros(rows, V, device="cuda")
+    x[:, 7] = x[:, 4000] = 2.0
+    x[:, 100:200] = -math.inf
+    lab = torch.full((rows,), 7, dtype=torch.int32, device="cuda")
+    s = ops.token_scores(x, lab, top_k=3, temperature=T, stats=True)
+    half = abs(math.log(0.5))
+    assert ((s.logprob + half).abs() <= 4 * R.U).all() and ((s.entropy - half).abs() <= 4 * R.U).all()
+    assert s.top_id[:, 0].eq(7).all() and s.top_id[:, 1].eq(4000).all() and s.top_logprob[:, 2].lt(-1e30).all()
+    one = torch.ones(rows, device="cuda")
+    want = torch.zeros(rows, V, dtype=torch.float64, device="cuda")
+    want[:, 7], want[:, 4000] = 0.5 / T, -0.5 / T
+    got = ops.token_scores_backward(x, lab, s.stats, s.entropy, one, None, temperature=T)
+    assert ((got - want).abs() <= 8 * R.U / T).all() and (got[:, 100:200] == 0).all()
+    got = ops.token_scores_backward(x, lab, s.stats, s.entropy, None, one, temperature=T)      # H is at its greatest
+    assert (got.abs() <= 8 * R.U / T).all() and (got[:, 100:200] == 0).all()
+    ids = torch.tensor([[7, 0]], dtype=torch.int32, device="cuda").expand(rows, 2).contiguous()
+    v = torch.tensor([[-half, -math.inf]], device="cuda").expand(rows, 2).contiguous()
+    want[:, 7], want[:, 4000] = 0.0, 0.0                       # p is the teacher's: half on 7, the rest on 4000
+    r = ops.distill_topk(x, ids, v, temperature=T, tail=True, grad=True, saved=True)
+    g = ops.distill_topk_backward(x, ids, v, r.saved, one, temperature=T, tail=True)
+    assert (r.row_loss.abs() <= 8 * R.U).all()
+    for d in (r.dlogits, g):
+        assert (d.abs() <= 8 * R.U / T).all() and (d[:, 100:200] == 0).all()
