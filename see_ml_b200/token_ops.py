@@ -4,8 +4,10 @@ their gradients. The entry points are described in include/seeml_b200.h.
 
 Logits are a [rows, vocab] tensor in f32, bf16 or f16 whose columns are contiguous; rows may be
 strided. Work is enqueued on torch's current stream of the logits' device and returns at once.
-These are plain functions, not autograd nodes: the gradient is a call of its own. Arguments that
-do not fit raise ``BackendError``.
+These are plain functions, not autograd nodes: the gradient is a call of its own, also of logits
+that require one (hand it on with ``logits.backward(dlogits)``). Writing into `out` counts as an
+in-place modification of it, which autograd refuses to overlook when a node has kept the tensor.
+Arguments that do not fit raise ``BackendError``.
 
     s = token_scores(teacher_logits, tokens, top_k=32, temperature=T)
     r = distill_topk(student_logits, s.top_id, s.top_logprob, row_weight=mask, scale=1 / n,
@@ -89,7 +91,7 @@ def _gradient(logits, out):
     return out, pitch
 
 
-def _call(fn, desc, device):
+def _call(fn, desc, device, out=None):
     stream = torch._C._cuda_getCurrentRawStream(device)      # current_stream() without building its object
     if torch._C._cuda_getDevice() == device:
         rc = fn(C.byref(desc), stream)
@@ -98,6 +100,8 @@ def _call(fn, desc, device):
             rc = fn(C.byref(desc), stream)
     if rc:
         raise L.BackendError(L.last_error())
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
 
 
 def _teacher(teacher_id, teacher_logprob, rows, device):
@@ -143,7 +147,7 @@ def token_scores_backward(logits, labels, stats, entropy, dlogprob, dentropy, *,
     g, g_pitch = _gradient(logits, out)
     d = L.TokenScoresGrad(logits.data_ptr(), lab, st, ent, dlp, dent, g.data_ptr(), rows, vocab, pitch, g_pitch, code,
                           temperature)
-    _call(L.lib().seeml_b200_token_scores_bwd, d, dev)
+    _call(L.lib().seeml_b200_token_scores_bwd, d, dev, out)
     return g
 
 
@@ -162,7 +166,7 @@ def distill_topk(logits, teacher_id, teacher_logprob, *, row_weight=None, scale=
     d = L.DistillTopk(logits.data_ptr(), tid, tlp, w, row_loss.data_ptr(), loss.data_ptr(),
                       keep.data_ptr() if saved else None, g.data_ptr() if g is not None else None, rows, vocab, pitch,
                       g_pitch, code, tcode, k, 1 if tail else 0, temperature, scale)
-    _call(L.lib().seeml_b200_distill_topk_fwd, d, dev)
+    _call(L.lib().seeml_b200_distill_topk_fwd, d, dev, out)
     return DistillLoss(loss, row_loss, keep, g)
 
 
@@ -175,5 +179,5 @@ def distill_topk_backward(logits, teacher_id, teacher_logprob, saved, drow_loss,
     g, g_pitch = _gradient(logits, out)
     d = L.DistillTopkGrad(logits.data_ptr(), tid, tlp, sv, up, g.data_ptr(), rows, vocab, pitch, g_pitch, code, tcode, k,
                           1 if tail else 0, temperature, 0)
-    _call(L.lib().seeml_b200_distill_topk_bwd, d, dev)
+    _call(L.lib().seeml_b200_distill_topk_bwd, d, dev, out)
     return g

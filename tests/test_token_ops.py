@@ -704,3 +704,29 @@ def test_the_lowest_temperature(backend_lib, rows):
     assert (r.row_loss.abs() <= 8 * R.U).all()
     for d in (r.dlogits, g):
         assert (d.abs() <= 8 * R.U / T).all() and (d[:, 100:200] == 0).all()
+
+
+@gpu
+def test_gradients_written_in_place_count_as_modifications(backend_lib):
+    """A node that kept the logits for its own backward pass does not compute with what the gradient left there."""
+    from see_ml_b200 import token_ops as ops
+    lab, one = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.ones(4, device="cuda")
+    ids, v = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.zeros(4, 1, device="cuda")
+    x = torch.zeros(4, 64, device="cuda")
+    s, r = ops.token_scores(x, lab, stats=True), ops.distill_topk(x, ids, v, saved=True)
+    for write in (lambda z: ops.token_scores_backward(z, lab, s.stats, s.entropy, one, None, out=z),
+                  lambda z: ops.distill_topk(z, ids, v, out=z),
+                  lambda z: ops.distill_topk_backward(z, ids, v, r.saved, one, out=z)):
+        leaf = torch.zeros(4, 64, device="cuda", requires_grad=True)
+        z = leaf + 1.0
+        loss = (z * z).sum()                                  # keeps z
+        before = z._version
+        write(z)
+        assert z._version > before
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+        with torch.inference_mode():                          # such tensors have no counter
+            write(torch.zeros(4, 64, device="cuda"))
+    before = x._version
+    ops.distill_topk(x, ids, v, grad=True)
+    assert x._version == before                               # a gradient of its own leaves the logits alone
