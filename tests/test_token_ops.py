@@ -730,3 +730,75 @@ def test_gradients_written_in_place_count_as_modifications(backend_lib):
     before = x._version
     ops.distill_topk(x, ids, v, grad=True)
     assert x._version == before                               # a gradient of its own leaves the logits alone
+
+
+# rows of 4 to 16 KiB of many rows go to a warp each, of few rows to blocks; both sides of the streamed kernels
+NOT_FINITE = [(F32, 2000), (BF16, 5000), (F16, 7001), (BF16, 40), (F16, 20011), (F32, 9001)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V", NOT_FINITE, ids=_ids)
+@pytest.mark.parametrize("copies,k", [(1, 4), (43, 2), (343, 16)])
+def test_scores_of_rows_that_are_not_finite(backend_lib, dtype, V, copies, k):
+    from see_ml_b200 import token_ops as ops
+    x = np.random.default_rng(V).standard_normal((8, V))
+    low = float(torch.finfo(dtype).min)
+    x[0] = -np.inf
+    x[1, V // 2] = np.nan
+    x[2, V - 1] = np.inf
+    x[3, 1:] = -np.inf
+    x[4, ::2] = low
+    x[5] = low
+    x[6, 1], x[6, V - 2], x[6, 3] = np.nan, np.nan, np.inf
+    t = torch.from_numpy(x).to(dtype).cuda()
+    labels = np.array([1, 0, 0, 0, 1, 3, 2, V], np.int32)
+    lab = torch.from_numpy(labels).cuda()
+    lp, h, tlp, tid = R.scores(_f64(t), labels, k, 0.5)
+    for s in _copies(ops.token_scores(t.repeat(copies, 1), lab.repeat(copies), top_k=k, temperature=0.5, stats=True), 8):
+        np.testing.assert_array_equal(s.top_id.cpu().numpy(), tid)
+        _close(s.logprob, lp, R.delta(V), F32, "logprob")
+        _close(s.entropy, h, 2 * (1 + math.log(V)) * R.delta(V), F32, "entropy")
+        _close(s.top_logprob, tlp, R.delta(V), F32, "top_logprob")
+    up = torch.ones(8 * copies, device="cuda")
+    many, stats, ent = t.repeat(copies, 1), s.stats.repeat(copies, 1), s.entropy.repeat(copies)
+    g = ops.token_scores_backward(many, lab.repeat(copies), stats, ent, up, up, temperature=0.5).view(copies, 8, V)
+    assert (g[:, 0] == 0).all() and g[:, [1, 2, 6, 7]].isnan().all() and (g[:, 3] == 0).all()
+    want, err = R.scores_grad(_f64(t)[4:6], labels[4:6], np.ones(2), np.ones(2), 0.5)
+    for c in {0, copies // 2, copies - 1}:
+        _close(g[c, 4:6], want, err, dtype, "dlogits")
+
+
+@gpu
+@pytest.mark.parametrize("dtype,V", NOT_FINITE + [(BF16, 140003)], ids=_ids)
+@pytest.mark.parametrize("copies", [1, 43])
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_of_rows_that_are_not_finite(backend_lib, dtype, V, copies, tail):
+    from see_ml_b200 import token_ops as ops
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((8, V))
+    ids, v = _teacher(rng, 8, V - 4, 6, F32)                   # the last four tokens are unnamed
+    i = ids.cpu().numpy()
+    low = float(torch.finfo(dtype).min)
+    x[0, V - 1] = np.nan
+    x[1, i[1, 2]] = np.nan
+    x[2, V - 2] = np.inf
+    x[3, i[3, 5]] = np.inf
+    x[4] = -np.inf
+    x[5] = low
+    x[6, V - 4:] = low
+    x[7, ::2] = -np.inf
+    x[7, i[7]] = 1.0
+    t = torch.from_numpy(x).to(dtype).cuda()
+    loss, lerr, grad, gerr = R.distill(_f64(t)[4:], i[4:], _f64(v)[4:], 1.0, tail)
+    many = t.repeat(copies, 1), ids.repeat(copies, 1), v.repeat(copies, 1)
+    r = ops.distill_topk(*many, tail=tail, grad=True, saved=True)
+    alone = ops.distill_topk(*many, tail=tail)
+    g = ops.distill_topk_backward(*many, r.saved, torch.ones(8 * copies, device="cuda"), tail=tail)
+    for c in {0, copies // 2, copies - 1}:
+        mine = slice(8 * c, 8 * c + 8)
+        for got in (r.row_loss[mine], alone.row_loss[mine]):
+            assert got[:4].isnan().all()
+            _close(got[4:], loss, lerr, F32, "row_loss")
+        for got in (r.dlogits[mine], g[mine]):
+            assert got[:4].isnan().all()
+            _close(got[4:], grad, gerr, dtype, "dlogits")
