@@ -249,8 +249,9 @@ int seeml_b200_token_scores_bwd(const seeml_b200_token_scores_grad* d, void* str
  *   row_loss[r] = l,   loss = scale * sum_r row_weight[r] * row_loss[r]
  * (there is no T^2; put it into scale). With dlogits the gradient of `loss` with respect to the
  * logits is written in the same pass, in the logits' type; dlogits may be the logits themselves.
- * A row of weight 0 is skipped, its logits are not read: row_loss 0, gradient 0. A token named twice counts with the sum
- * of its entries' q. An entry with a token >= vocab is not dereferenced; it makes the row NaN. */
+ * A row of weight 0 is skipped, its logits are not read: row_loss 0, gradient 0. A token named
+ * twice has a term per entry in the loss, and the sum of its entries' q in the gradient. An entry
+ * with a token >= vocab is not dereferenced; it makes the row NaN. */
 typedef struct seeml_b200_distill_topk {
   const void* logits;
   const int32_t* teacher_id;     /* [rows, top_k] */

@@ -7,8 +7,10 @@
 //   dl/dx_j = (p_j Q - q_j - [j unnamed] q_t p_j / p_t) / T,   Q = sum q + q_t.
 // Unnamed tokens share one factor, A exp((x_j - mt) / T), so the gradient costs one exponential and
 // one product per element behind the row's sums. Named tokens are left out of those sums: p_t comes
-// without a difference, however little of the student's mass is left. HBM bounds all of it: one
-// read of the logits, and one write where the gradient is wanted.
+// without a difference, however little of the student's mass is left. HBM bounds it: one read of the
+// logits, and one write where the gradient is wanted; the step reads most of a row that one block
+// streams a second time, partly out of L2. In 16 bits the step's two exponentials per element come
+// near that bound too.
 #include "token_rows.cuh"
 
 namespace seeml_b200 {
@@ -608,7 +610,8 @@ DistillArgs distill_args(const seeml_b200_distill_topk& d) {
 }
 // Bytes of the words that mark the named tokens of a share.
 size_t named_bytes(uint64_t vecs, int threads) { return (vecs + kBatch * threads - 1) / (kBatch * threads) * threads * 4; }
-// Of a row in one block: six blocks live on an SM (16384 x 32000 f32, step: 700 us; 66 KiB and three blocks 756 us).
+// Of a row in one block: five blocks live on an SM when their shares are full, six of 16384 x 32000 f32, whose shares hold
+// 31 KiB (step: 700 us; with 66 KiB and three blocks 768 us).
 constexpr uint64_t kMostParked = 34u << 10;
 
 }  // namespace

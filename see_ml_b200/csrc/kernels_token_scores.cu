@@ -2,9 +2,11 @@
 // and the most likely tokens, and the gradient of the first two.
 //
 // A few operations per element over [rows, vocab] logits that are read once: HBM bounds the
-// forward call, and reading and writing them the backward one. At 16384 x 32000 f32 with 16
-// alternatives the forward call takes 318 us, the copy rate; what a block then spends on the selection
-// of the alternatives, other blocks on the SM hide.
+// forward call, and reading and writing them the backward one. At 16384 x 32000 f32 the forward
+// call takes 291 us, with 16 alternatives 322 us (median of replays; 362 us in a run of calls whose
+// inputs change), 321 us being the copy rate. What a block spends on the selection of the
+// alternatives, other blocks on the SM hide where rows are long; rows of up to 64 KiB are bound by it:
+// 20000 x 1000 f32 takes 17 us without, 49 us with 16, 220 us with 128 of them.
 #include "token_rows.cuh"
 
 namespace seeml_b200 {
@@ -369,8 +371,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_scores_stream_kernel(seeml_
   Label lab{-1, 0.0f};
   if (threadIdx.x == kThreads - 1) lab = load_label(d, r, sh);
   // While this row's selection leaves the memory idle, the start of a row that comes next is brought into L2: 64 KiB of
-  // the row three blocks per SM ahead (16384 x 32000 f32 with 16 alternatives: 371 us without, 349 us with; 128 KiB or
-  // one to four blocks per SM ahead gave 356-381).
+  // the row three blocks per SM ahead (16384 x 32000 f32 with 16 alternatives: 360 us without, 322 us with).
   if (threadIdx.x == 32 && r + 3 * kSMs < d.rows) prefetch_row(static_cast<const T*>(d.logits) + (r + 3 * kSMs) * d.row_stride, V);
   publish_max(ss, a.m);
   const uint32_t key = threadIdx.x < sh.n ? order_key(a.m) : 0u;
@@ -618,8 +619,8 @@ __global__ void __launch_bounds__(32 * kRowWarps) token_scores_rows_kernel(seeml
 
 // ---- gradient of the scores ----------------------------------------------------------------------
 // dlogits = e (a + b y) with e = 2^y, y = (x - max) log2(e) / T: the row's factors are a few numbers.
-// One block per 32 KiB of a row or one warp per 4 KiB, eight vectors in flight per thread (8192 x 32000 f32: 304 us; four
-// vectors 361 us).
+// One block per 32 KiB of a row or one warp per 4 KiB, eight vectors in flight per thread (8192 x 32000 f32: 324 us; four
+// vectors 389 us).
 constexpr int kGradVecs = 8;
 struct GradRow {
   float m, a, b;

@@ -372,9 +372,9 @@ __device__ __forceinline__ double ln_sum(float S) {
 // Two sources of batches. Streamed: a call of many rows gives each row to one block that reads it
 // straight into registers, the next batch in flight behind the one being summed; several blocks
 // live on an SM, so that the ends of rows hide behind the middle of others, and nothing couples the
-// blocks (a cluster has to find room for all its blocks at once, which left SMs idle: scores of
-// 16384 x 32000 f32 took 635 us parked in clusters of two, 392 us streamed). Parked: the block's
-// share is copied to shared memory, where it stays for what comes after the sums.
+// blocks (a cluster has to find room for all its blocks at once, which leaves SMs idle: scores of
+// 16384 x 32000 f32 with 16 alternatives take 672 us parked in clusters of two, 322 us streamed).
+// Parked: the block's share is copied to shared memory, where it stays for what comes after the sums.
 // Vector i of the row, -inf beyond the row's ends.
 template <class T, int NT>
 __device__ __forceinline__ uint4 row_vec(const Share<T, NT>& sh, uint32_t i) {
@@ -573,7 +573,9 @@ inline uint64_t row_vecs(uint64_t vocab, uint64_t elem) {          // at most, w
   return (vocab + 2 * (per - 1)) / per;
 }
 // Blocks per parked row, each with at most `most` bytes of it so that several live on an SM and one copies while others
-// compute; a call of few rows is spread further, down to 8 KiB a block, until it covers the SMs.
+// compute; a call of few rows is spread further, blocks of more than 8 KiB being halved, until it covers the SMs. The number
+// of blocks is a power of two, so a row just above a limit leaves its shares half empty: distillation steps of equal bytes
+// take 803 us with 33790 tokens of bf16 (two shares of 33 KiB) and 970 us with 36862 (four of 18 KiB).
 struct Split {
   uint32_t blocks, share;      // share in 16-byte vectors
 };
@@ -614,7 +616,16 @@ int launch_rows(uint64_t rows, uint32_t blocks, bool cluster, int threads, size_
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, Kernel, args...) == cudaSuccess ? 1 : -1;
 }
-// Rows from which on a row per block keeps all SMs busy.
+// Rows from which on a row has one block to itself, or a warp where it is short. One number for all operators; in us by
+// clusters and by a block or warp a row, with 8 alternatives (2 of the short rows) or 16 entries:
+//   rows                             64          148          250          296          400          777
+//   scores, 32000 f32          9.2   7.6   10.5   8.0   19.9   9.3   20.3   9.4   20.8  11.4   39.7  20.7
+//   loss, 32000 f32            7.3   7.5    8.9   7.7   12.2   9.2   13.4   9.3   15.6  10.7   25.1  19.3
+//   step, 131072 bf16         12.6  18.2   22.3  19.5   37.8  32.1   42.8  35.2   54.8  52.0   96.6  92.5
+//   scores, 2000 f32           7.0   8.0    6.8   8.4    7.1   8.1    6.9   8.2    7.3   8.4    9.1   8.6
+//   step, 2000 f32             6.4  10.5    7.3  10.6    7.1  10.8    7.2  10.9    7.4  10.9    7.7  10.6
+//   backward, 1000 f32         4.0   5.5    4.0   5.6    4.3   5.9    4.3   5.6    4.3   6.1    5.7   5.8
+// Long rows would cross over near 148 rows, short ones near 777.
 constexpr uint64_t kManyRows = 2 * kSMs;
 
 }  // namespace
